@@ -1,0 +1,105 @@
+// paged.cuh — index arithmetic of the paged KV cache, shared by its kernels and by the host test
+// that walks it (every division of work and every place in a pool is computed here).
+#pragma once
+
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+
+#ifdef __CUDACC__
+#define QA_HD __host__ __device__ __forceinline__
+#else
+#define QA_HD inline
+#endif
+
+namespace qattn {
+
+// Codes left in the error block for page tables, lengths and positions read on the device
+// (reported as QA_ERR_INVALID; every other code is an expired wait).
+constexpr int PAGED_BAD_LENGTH = 61, PAGED_BAD_PAGE = 62, PAGED_BAD_POSITION = 63, PAGED_BAD_SEQ = 64;
+
+// A length as the kernels use it: one outside its table (cols pages of 1 << shift rows) is 0.
+QA_HD int paged_length(int len, int cols, int shift) { return len < 0 || len > cols << shift ? 0 : len; }
+
+// Page of a new row that its sequence `seq` holds as its len-th, or -1 with *code set (0: a padded row).
+QA_HD int paged_place(int len, int seq, int pos, int n_seqs, int cols, int shift, int rope_rows, int n_pages,
+                      const int* table, int* code) {
+    *code = 0;
+    if (len == 0) return -1;
+    if ((unsigned)pos >= (unsigned)rope_rows) { *code = PAGED_BAD_POSITION; return -1; }
+    if ((unsigned)seq >= (unsigned)n_seqs) { *code = PAGED_BAD_SEQ; return -1; }
+    const unsigned col = ((unsigned)len - 1u) >> shift;
+    if (col >= (unsigned)cols) { *code = PAGED_BAD_LENGTH; return -1; }
+    const int page = table[(size_t)seq * cols + col];
+    if ((unsigned)page >= (unsigned)n_pages) { *code = PAGED_BAD_PAGE; return -1; }
+    return page;
+}
+
+// ---- even split of an attention call --------------------------------------------------------------
+// The 16-row blocks of all units (layer, row, KV head), laid end to end in that order, are cut
+// into `ctas` equal ranges. start[b] = blocks of one head of rows [0, b), b <= n.
+constexpr int PAGED_BLK = 16;                 // cache rows per block (the smallest page)
+
+struct PagedUnit { int l, b, kh, nblk; long long off; };   // blocks [off, off + nblk) of the call
+
+struct PagedSplit {
+    long long total;                          // blocks of the call
+    int ctas;                                 // ranges in use
+    QA_HD long long begin(int c) const { return (long long)c * total / ctas; }
+    // range that holds block g: the largest c with begin(c) <= g
+    QA_HD int range_of(long long g) const { return (int)(((g + 1) * ctas - 1) / total); }
+};
+
+QA_HD PagedSplit paged_split(long long total, int max_ctas, int min_blocks) {
+    PagedSplit s;
+    s.total = total;
+    const long long fit = total / min_blocks;
+    s.ctas = fit < 1 ? 1 : fit < max_ctas ? (int)fit : max_ctas;
+    return s;
+}
+
+QA_HD PagedUnit paged_unit_of(const int* start, int n, int hkv, long long g) {
+    const long long layer_blocks = (long long)hkv * start[n];
+    PagedUnit u;
+    u.l = (int)(g / layer_blocks);
+    const long long r = g - u.l * layer_blocks;
+    int lo = 0, hi = n;                       // largest b with hkv * start[b] <= r (rows of length 0 have no width)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if ((long long)hkv * start[mid] <= r) lo = mid; else hi = mid;
+    }
+    u.b = lo;
+    u.nblk = start[lo + 1] - start[lo];
+    const long long rr = r - (long long)hkv * start[lo];
+    u.kh = (int)(rr / u.nblk);
+    u.off = g - (rr - (long long)u.kh * u.nblk);
+    return u;
+}
+
+// The unit after u; not called past the last one.
+QA_HD void paged_next_unit(const int* start, int n, int hkv, PagedUnit& u) {
+    u.off += u.nblk;
+    if (++u.kh == hkv) {
+        u.kh = 0;
+        do {
+            if (++u.b == n) { u.b = 0; ++u.l; }
+            u.nblk = start[u.b + 1] - start[u.b];
+        } while (u.nblk == 0);
+    }
+}
+
+// ---- eviction order -------------------------------------------------------------------------------
+// Larger weight <=> larger key; -0 equals 0; NaN is the lowest.
+QA_HD uint32_t evict_key(float w) {
+    if (w != w) return 0u;
+    w += 0.f;
+    uint32_t b;
+#ifdef __CUDA_ARCH__
+    b = __float_as_uint(w);
+#else
+    std::memcpy(&b, &w, 4);
+#endif
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+}  // namespace qattn

@@ -39,8 +39,9 @@ struct qa_ctx {
     cudaStream_t stream = nullptr;
     KVLayout kv{};
     float* norms = nullptr;                // [L][2][128]
-    float* cosines = nullptr;              // [ctx][64]
+    float* cosines = nullptr;              // [rope_rows][64]
     float* sines = nullptr;
+    int rope_rows = 0;                     // positions of the tables: context, or more (qa_rope_positions)
     std::vector<int> pos;                  // committed position per sequence
     std::vector<std::vector<int>> appended;  // per sequence, per layer: rows written through
     void* proj_scratch = nullptr;          // the tensor-core projections' split input rows (project_mma.cu)
@@ -139,6 +140,8 @@ int fail(qa_ctx* c, int status, const char* fmt, ...) {
 int cuda_fail(qa_ctx* c, cudaError_t e, const char* what) {
     return fail(c, e == cudaErrorMemoryAllocation ? QA_ERR_OOM : QA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
+
+int device_error(qa_ctx* ctx, int code, const char* which);
 
 #define QA_CUDA(call)                                                  \
     do {                                                               \
@@ -253,7 +256,7 @@ int io_host_call(qa_ctx* ctx, int seq, int layer, int n_layers, const IoCall& c,
                 ctx->pos[seq] = 0;
                 std::fill(ctx->appended[seq].begin(), ctx->appended[seq].end(), 0);
             }
-            return fail(ctx, QA_ERR_TIMEOUT, "a device-side wait expired (code %d); the call's results are invalid", code);
+            return device_error(ctx, code, "the call's results are invalid");
         }
         return QA_OK;
     };
@@ -353,14 +356,59 @@ int make_kv_map(qa_ctx* ctx) {
     return QA_OK;
 }
 
-// Reads and clears the device error flag of the bounded waits.
+// RoPE tables of positions [0, n) exactly as core.cpp:288 computes them (FP64 angle, FP64 cos/sin,
+// FP32 store), in place of the context's present ones. On failure the present tables stay.
+int make_rope_tables(qa_ctx* ctx, int n) {
+    std::vector<float> cs, sn;
+    try {
+        cs.resize((size_t)n * 64);
+        sn.resize(cs.size());
+    } catch (const std::bad_alloc&) {
+        return fail(ctx, QA_ERR_OOM, "no host memory for %d RoPE positions", n);
+    }
+    double base[64];
+    for (int j = 0; j < 64; ++j) base[j] = std::pow(ctx->cfg.rope_theta, 2.0 * j / D);
+    for (int p = 0; p < n; ++p)
+        for (int j = 0; j < 64; ++j) {
+            const double angle = p / base[j];
+            cs[(size_t)p * 64 + j] = (float)std::cos(angle);
+            sn[(size_t)p * 64 + j] = (float)std::sin(angle);
+        }
+    float *dc = nullptr, *ds = nullptr;
+    const size_t bytes = cs.size() * sizeof(float);
+    cudaError_t e = cudaMalloc(&dc, bytes);
+    if (e == cudaSuccess) e = cudaMalloc(&ds, bytes);
+    if (e == cudaSuccess) e = cudaMemcpy(dc, cs.data(), bytes, cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = cudaMemcpy(ds, sn.data(), bytes, cudaMemcpyHostToDevice);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        cudaFree(dc); cudaFree(ds);
+        return cuda_fail(ctx, e, "RoPE tables");
+    }
+    cudaFree(ctx->cosines); cudaFree(ctx->sines);
+    ctx->cosines = dc; ctx->sines = ds; ctx->rope_rows = n;
+    return QA_OK;
+}
+
+// The status and message of a code that the device left in the error block.
+int device_error(qa_ctx* ctx, int code, const char* which) {
+    switch (code) {
+        case PAGED_BAD_LENGTH: return fail(ctx, QA_ERR_INVALID, "a paged call met a length outside its table (code %d)", code);
+        case PAGED_BAD_PAGE: return fail(ctx, QA_ERR_INVALID, "a paged call met a page id outside the pool (code %d)", code);
+        case PAGED_BAD_POSITION: return fail(ctx, QA_ERR_INVALID, "a paged append met a position outside the RoPE tables (code %d)", code);
+        case PAGED_BAD_SEQ: return fail(ctx, QA_ERR_INVALID, "a paged append met a sequence outside the table (code %d)", code);
+        default: return fail(ctx, QA_ERR_TIMEOUT, "a device-side wait expired (code %d); %s", code, which);
+    }
+}
+
+// Reads and clears the device error flag of the bounded waits and the paged calls.
 int check_device_error(qa_ctx* ctx) {
     int code = 0;
     QA_CUDA(cudaMemcpyAsync(&code, ctx->error, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
     QA_CUDA(cudaStreamSynchronize(ctx->stream));
     if (code) {
         QA_CUDA(cudaMemsetAsync(ctx->error, 0, sizeof(int), ctx->stream));
-        return fail(ctx, QA_ERR_TIMEOUT, "a device-side wait expired (code %d); results of the last calls are invalid", code);
+        return device_error(ctx, code, "results of the last calls are invalid");
     }
     return QA_OK;
 }
@@ -438,18 +486,7 @@ int qa_create(const qa_config* cfg, qa_ctx** out) {
     if (cudaMalloc(&ctx->kv.base, kv_bytes) != cudaSuccess) return cleanup(QA_ERR_OOM);
     if (cudaMemset(ctx->kv.base, 0, kv_bytes) != cudaSuccess) return cleanup(QA_ERR_CUDA);
 
-    // RoPE tables exactly as core.cpp:288 computes them (FP64 angle, FP64 cos/sin, FP32 store).
-    std::vector<float> cs((size_t)c.context * 64), sn(cs.size());
-    for (int p = 0; p < c.context; ++p)
-        for (int j = 0; j < 64; ++j) {
-            const double angle = p / std::pow(c.rope_theta, 2.0 * j / D);
-            cs[(size_t)p * 64 + j] = (float)std::cos(angle);
-            sn[(size_t)p * 64 + j] = (float)std::sin(angle);
-        }
-    if (cudaMalloc(&ctx->cosines, cs.size() * sizeof(float)) != cudaSuccess) return cleanup(QA_ERR_OOM);
-    if (cudaMalloc(&ctx->sines, sn.size() * sizeof(float)) != cudaSuccess) return cleanup(QA_ERR_OOM);
-    if (cudaMemcpy(ctx->cosines, cs.data(), cs.size() * sizeof(float), cudaMemcpyHostToDevice) != cudaSuccess) return cleanup(QA_ERR_CUDA);
-    if (cudaMemcpy(ctx->sines, sn.data(), sn.size() * sizeof(float), cudaMemcpyHostToDevice) != cudaSuccess) return cleanup(QA_ERR_CUDA);
+    if (const int st = make_rope_tables(ctx, c.context)) return cleanup(st);
 
     std::vector<float> ones((size_t)c.n_layers * 2 * D, 1.0f);
     if (cudaMalloc(&ctx->norms, ones.size() * sizeof(float)) != cudaSuccess) return cleanup(QA_ERR_OOM);
@@ -1071,7 +1108,7 @@ int project_call(qa_ctx* ctx, int n_mats, const uint16_t* const* w, const int* r
     if (const int code = h_err[ERR_CODE]) {
         QA_CUDA(cudaMemsetAsync(ctx->error + ERR_CODE, 0, sizeof(int), ctx->stream));
         QA_CUDA(cudaStreamSynchronize(ctx->stream));
-        return fail(ctx, QA_ERR_TIMEOUT, "a device-side wait expired (code %d); results of the last calls are invalid", code);
+        return device_error(ctx, code, "results of the last calls are invalid");
     }
     return QA_OK;
 }
@@ -1464,3 +1501,152 @@ int qa_comm_join(qa_ctx* ctx) {
 }
 
 }  // extern "C"
+
+// ---- paged KV cache (kv_paged.cu, attn_paged.cu, evict_paged.cu) ----------------------------------
+namespace {
+bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+// Checks the pool and one of its tables and fills the kernels' view of the pool.
+int check_pages(qa_ctx* ctx, const qa_pages* p, const int* table, int cols, bool weights, PagedKV* kv) {
+    if (!p || !p->kv || !table) return fail(ctx, QA_ERR_INVALID, "null page pool or table");
+    if (p->n_pages < 1) return fail(ctx, QA_ERR_INVALID, "%d pages", p->n_pages);
+    int shift = 4;
+    while (shift < 9 && (1 << shift) != p->page_rows) ++shift;
+    if ((1 << shift) != p->page_rows)
+        return fail(ctx, QA_ERR_INVALID, "page of %d rows (16, 32, 64, 128, 256 or 512)", p->page_rows);
+    if (!aligned(p->kv, 16) || !aligned(p->weights, 16) || !aligned(table, 4))
+        return fail(ctx, QA_ERR_INVALID, "page pool or table not aligned (16 bytes, 4 bytes)");
+    if (weights && !p->weights) return fail(ctx, QA_ERR_INVALID, "the pages hold no attention weights");
+    if (cols < 1 || cols > QA_MAX_PAGED_ROWS / p->page_rows)
+        return fail(ctx, QA_ERR_INVALID, "table of %d columns (1..%d)", cols, QA_MAX_PAGED_ROWS / p->page_rows);
+    kv->base = reinterpret_cast<__half*>(p->kv);
+    kv->weights = p->weights;
+    kv->n_pages = p->n_pages; kv->shift = shift; kv->layers = ctx->cfg.n_layers; kv->hkv = ctx->hkv;
+    return QA_OK;
+}
+
+int check_paged_batch(qa_ctx* ctx, int n) {
+    if (n < 1 || n > QA_MAX_PAGED_BATCH)
+        return fail(ctx, QA_ERR_INVALID, "batch of %d sequences (1..%d)", n, QA_MAX_PAGED_BATCH);
+    return QA_OK;
+}
+
+int check_tensor(qa_ctx* ctx, const void* p, const char* name) {
+    if (!p) return fail(ctx, QA_ERR_INVALID, "null %s", name);
+    if (!aligned(p, ctx->cfg.io_host ? 4 : 16)) return fail(ctx, QA_ERR_INVALID, "%s is not aligned", name);
+    return QA_OK;
+}
+
+int check_ints(qa_ctx* ctx, const void* p, const char* name) {
+    if (!p || !aligned(p, 4)) return fail(ctx, QA_ERR_INVALID, "%s is null or not aligned", name);
+    return QA_OK;
+}
+}  // namespace
+
+int qa_rope_positions(qa_ctx* ctx, int n) {
+    if (!ctx) return QA_ERR_INVALID;
+    if (n < 1 || n > QA_MAX_PAGED_ROWS) return fail(ctx, QA_ERR_INVALID, "%d RoPE positions (1..%d)", n, QA_MAX_PAGED_ROWS);
+    if (n <= ctx->rope_rows) return QA_OK;
+    QA_CUDA(cudaSetDevice(ctx->cfg.device));
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    QA_CUDA(cudaStreamIsCapturing(ctx->stream, &capturing));
+    if (capturing != cudaStreamCaptureStatusNone)
+        return fail(ctx, QA_ERR_STATE, "the context's stream is capturing");
+    QA_CUDA(cudaStreamSynchronize(ctx->stream));
+    ctx->last_fused_step = false;
+    return make_rope_tables(ctx, n);
+}
+
+int qa_paged_append(qa_ctx* ctx, const qa_pages* pages, const int* table, int n_seqs, int table_cols,
+                    const int* row_seq, const int* row_len, const int* row_pos, int n, int layer, int n_layers,
+                    const float* q_pre, const float* k_pre, const float* v, float* q_out) {
+    if (!ctx) return QA_ERR_INVALID;
+    int st;
+    PagedAppendArgs a{};
+    if ((st = check_layers(ctx, layer, n_layers)) || (st = check_pages(ctx, pages, table, table_cols, false, &a.kv))) return st;
+    if (n < 1 || n > QA_MAX_PAGED_ROWS) return fail(ctx, QA_ERR_INVALID, "%d new rows (1..%d)", n, QA_MAX_PAGED_ROWS);
+    if (n_seqs < 1) return fail(ctx, QA_ERR_INVALID, "table of %d sequences", n_seqs);
+    if (!row_seq && n > n_seqs) return fail(ctx, QA_ERR_INVALID, "%d new rows without row_seq for %d sequences", n, n_seqs);
+    if (!aligned(row_seq, 4)) return fail(ctx, QA_ERR_INVALID, "row_seq is not aligned");
+    if ((st = check_ints(ctx, row_len, "row_len")) || (st = check_ints(ctx, row_pos, "row_pos")) ||
+        (st = check_tensor(ctx, q_pre, "q_pre")) || (st = check_tensor(ctx, k_pre, "k_pre")) || (st = check_tensor(ctx, v, "v")) ||
+        (q_out && (st = check_tensor(ctx, q_out, "q_out"))))
+        return st;
+    QA_CUDA(cudaSetDevice(ctx->cfg.device));
+    a.table = table; a.n_seqs = n_seqs; a.cols = table_cols;
+    a.row_seq = row_seq; a.row_len = row_len; a.row_pos = row_pos; a.n = n; a.rope_rows = ctx->rope_rows;
+    a.norms = ctx->norms; a.cosines = ctx->cosines; a.sines = ctx->sines; a.eps = ctx->cfg.norm_eps; a.error = ctx->error;
+    const size_t qn = (size_t)n * ctx->hq * D, kn = (size_t)n * ctx->hkv * D;
+    IoCall c;
+    c.in[0] = q_pre; c.in[1] = k_pre; c.in[2] = v; c.in_floats[0] = qn; c.in_floats[1] = kn; c.in_floats[2] = kn;
+    c.out[0] = q_out; c.out_floats[0] = q_out ? qn : 0;
+    return run_call(ctx, -1, layer, n_layers, c, [&](int l0, int nl, const float* const* din, float* const* dout) {
+        a.q_pre = din[0]; a.k_pre = din[1]; a.v_pre = din[2]; a.q_out = q_out ? dout[0] : nullptr;
+        a.layer0 = l0; a.n_layers = nl;
+        launch_paged_append(a, ctx->stream);
+        return after_launch(ctx, -1, "paged_append");
+    });
+}
+
+int qa_paged_workspace(const qa_ctx* ctx, int n, int n_layers, int max_rows, int add_weights, size_t* bytes) {
+    if (!ctx || !bytes) return QA_ERR_INVALID;
+    if (n < 1 || n > QA_MAX_PAGED_BATCH || n_layers < 1 || n_layers > ctx->cfg.n_layers || max_rows < 1 ||
+        max_rows > QA_MAX_PAGED_ROWS)
+        return QA_ERR_INVALID;
+    *bytes = paged_attn_workspace(n, n_layers, ctx->hkv, max_rows, add_weights != 0);
+    return QA_OK;
+}
+
+int qa_paged_attn(qa_ctx* ctx, const qa_pages* pages, const int* table, int table_cols, const int* lengths, int n,
+                  int layer, int n_layers, const float* q, float* out, int add_weights, void* workspace,
+                  size_t workspace_bytes) {
+    if (!ctx) return QA_ERR_INVALID;
+    int st;
+    PagedAttnArgs a{};
+    if ((st = check_layers(ctx, layer, n_layers)) ||
+        (st = check_pages(ctx, pages, table, table_cols, add_weights != 0, &a.kv)) || (st = check_paged_batch(ctx, n)) ||
+        (st = check_ints(ctx, lengths, "lengths")) || (st = check_tensor(ctx, q, "q")) || (st = check_tensor(ctx, out, "out")))
+        return st;
+    const size_t need = paged_attn_workspace(n, n_layers, ctx->hkv, table_cols * pages->page_rows, add_weights != 0);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+        return fail(ctx, QA_ERR_INVALID, "workspace of %zu bytes (null, not 16-byte aligned, or below the %zu needed)",
+                    workspace_bytes, need);
+    QA_CUDA(cudaSetDevice(ctx->cfg.device));
+    a.table = table; a.cols = table_cols; a.lengths = lengths; a.n = n; a.add_weights = add_weights != 0;
+    a.records = static_cast<float*>(workspace);
+    a.logits = reinterpret_cast<float*>(static_cast<char*>(workspace) + paged_attn_record_bytes());
+    a.error = ctx->error;
+    const size_t qn = (size_t)n * ctx->hq * D;
+    IoCall c;
+    c.in[0] = q; c.in_floats[0] = qn;
+    c.out[0] = out; c.out_floats[0] = qn;
+    c.inputs_read_once = decode_inputs_read_once(n_layers, n, ctx->hkv);
+    return run_call(ctx, -1, layer, n_layers, c, [&](int l0, int nl, const float* const* din, float* const* dout) {
+        a.q = din[0]; a.out = dout[0]; a.layer0 = l0; a.n_layers = nl;
+        const cudaError_t e = launch_paged_attn(a, ctx->stream);
+        if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, e, "paged_attn"); }
+        return after_launch(ctx, -1, "paged_attn");
+    });
+}
+
+int qa_paged_evict(qa_ctx* ctx, const qa_pages* pages, const int* src_table, int src_cols, const int* dst_table,
+                   int dst_cols, const int* lengths, int* new_lengths, int n, int keep, int recent, int* kept) {
+    if (!ctx) return QA_ERR_INVALID;
+    int st;
+    PagedEvictArgs a{};
+    if ((st = check_pages(ctx, pages, src_table, src_cols, true, &a.kv)) ||
+        (st = check_pages(ctx, pages, dst_table, dst_cols, true, &a.kv)) || (st = check_paged_batch(ctx, n)) ||
+        (st = check_ints(ctx, lengths, "lengths")) || (st = check_ints(ctx, new_lengths, "new_lengths")) ||
+        (st = check_ints(ctx, kept, "kept")))
+        return st;
+    if (keep < 1 || keep > dst_cols * pages->page_rows)
+        return fail(ctx, QA_ERR_INVALID, "keep %d rows (1..%d)", keep, dst_cols * pages->page_rows);
+    if (recent < 0 || recent > keep) return fail(ctx, QA_ERR_INVALID, "recent %d outside [0,%d]", recent, keep);
+    QA_CUDA(cudaSetDevice(ctx->cfg.device));
+    a.src_table = src_table; a.src_cols = src_cols; a.dst_table = dst_table; a.dst_cols = dst_cols;
+    a.lengths = lengths; a.new_lengths = new_lengths; a.n = n; a.keep = keep; a.recent = recent; a.kept = kept;
+    a.error = ctx->error;
+    const cudaError_t e = launch_paged_evict(a, ctx->stream);
+    if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, e, "paged_evict"); }
+    return after_launch(ctx, -1, "paged_evict");
+}

@@ -9,6 +9,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "paged.cuh"
+
 namespace qattn {
 
 constexpr int D = 128;          // head_dim
@@ -195,6 +197,57 @@ void launch_project(ProjectArgs a, cudaStream_t s);
 constexpr int GEMM_CHUNK_ROWS = 512, GEMM_MAX_COLS = 8192;
 size_t project_gemm_scratch_bytes();
 int launch_project_gemm(const ProjectArgs& a, void* scratch, int* error, cudaStream_t s);
+
+// ---- paged KV cache (kv_paged.cu, attn_paged.cu, evict_paged.cu) -------------------------------
+// Pool of pages, each one block [layer][K|V][kv_head][row][128] FP16 with 1 << shift rows, and the
+// accumulated attention weights [page][layer][kv_head][row] FP32 (null: not kept).
+struct PagedKV {
+    __half* base = nullptr;
+    float* weights = nullptr;
+    int n_pages = 0, shift = 0, layers = 0, hkv = 0;
+    __device__ __forceinline__ __half* row(int page, int layer, int kv, int head, int r) const {
+        return base + ((((((size_t)page * layers + layer) * 2 + kv) * hkv + head) << shift) + r) * D;
+    }
+    __device__ __forceinline__ float* weight(int page, int layer, int head, int r) const {
+        return weights + ((((size_t)page * layers + layer) * hkv + head) << shift) + r;
+    }
+    __device__ __forceinline__ bool has(int page) const { return (unsigned)page < (unsigned)n_pages; }
+};
+struct PagedAppendArgs {
+    const float* q_pre; const float* k_pre; const float* v_pre; float* q_out;   // q_out may be null
+    PagedKV kv;
+    const int* table; int n_seqs, cols;
+    const int* row_seq; const int* row_len; const int* row_pos;                 // row_seq may be null
+    int n, layer0, n_layers, rope_rows;
+    const float* norms; const float* cosines; const float* sines;
+    float eps;
+    int* error;
+};
+void launch_paged_append(const PagedAppendArgs& a, cudaStream_t s);
+
+struct PagedAttnArgs {
+    const float* q; float* out;               // [n_layers][n][2 * hkv][128]
+    PagedKV kv;
+    const int* table; int cols; const int* lengths;
+    int n, layer0, n_layers, add_weights;
+    float* records;                           // workspace: [ctas][2][PARTIAL_FLOATS]
+    float* logits;                            // workspace with add_weights: [16-row block][16][2]
+    int* error;
+};
+constexpr int MAX_PAGED_BATCH = 1024;
+size_t paged_attn_workspace(int n, int n_layers, int hkv, int max_rows, bool add_weights);
+size_t paged_attn_record_bytes();
+cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s);
+
+struct PagedEvictArgs {
+    PagedKV kv;
+    const int* src_table; int src_cols; const int* dst_table; int dst_cols;
+    const int* lengths; int* new_lengths;
+    int n, keep, recent;
+    int* kept;                                // [n][layers][hkv][keep]
+    int* error;
+};
+cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t s);
 
 // Looks up, for `device` and its current context, the device address of the fixed scratch array
 // behind qa_attn_decode_noalloc (attn_decode_noalloc.cu). Makes `device` current.

@@ -21,6 +21,7 @@ STATUS = {1: "invalid argument", 2: "context capacity exceeded", 3: "invalid sta
 QA_ERR_INVALID, QA_ERR_CAPACITY, QA_ERR_STATE, QA_ERR_CUDA = 1, 2, 3, 4
 QA_ERR_NCCL, QA_ERR_TIMEOUT, QA_ERR_OOM, QA_ERR_UNSUPPORTED = 5, 6, 7, 8
 PREFIX_CHUNK = 512
+MAX_PAGED_BATCH, MAX_PAGED_ROWS = 1024, 1 << 20
 MAX_DECODE_ROWS = 4
 MAX_BATCH = 64
 HEAD_DIM = 128
@@ -40,6 +41,12 @@ class Config(ctypes.Structure):
                 ("kv_head_begin", ctypes.c_int), ("kv_head_count", ctypes.c_int),
                 ("rope_theta", ctypes.c_double), ("norm_eps", ctypes.c_float), ("device", ctypes.c_int),
                 ("io_host", ctypes.c_int)]
+
+
+class Pages(ctypes.Structure):
+    """qa_pages: the caller's pool of KV pages (device addresses; weights 0 or None: not kept)."""
+    _fields_ = [("kv", ctypes.c_void_p), ("weights", ctypes.c_void_p), ("n_pages", ctypes.c_int),
+                ("page_rows", ctypes.c_int)]
 
 
 _lib = None
@@ -115,6 +122,19 @@ _SIGNATURES = {
                                        ctypes.c_int, ctypes.c_void_p]),
     "qa_project_group_gemm": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
                                              ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+    "qa_rope_positions": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int]),
+    "qa_paged_append": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Pages), ctypes.c_void_p, ctypes.c_int,
+                                       ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+                                       ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                       ctypes.c_void_p]),
+    "qa_paged_workspace": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                          ctypes.POINTER(ctypes.c_size_t)]),
+    "qa_paged_attn": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Pages), ctypes.c_void_p, ctypes.c_int,
+                                     ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                     ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t]),
+    "qa_paged_evict": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Pages), ctypes.c_void_p, ctypes.c_int,
+                                      ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+                                      ctypes.c_int, ctypes.c_int, ctypes.c_void_p]),
     "qa_synth_fill": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                      ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float,
                                      ctypes.c_float, ctypes.c_void_p]),
@@ -284,6 +304,36 @@ class Context:
     def commit_batch(self, seqs):
         arr, n = self._seq_array(seqs)
         self._check(lib().qa_commit_batch(self._h, arr, n))
+
+    # -- paged KV cache (addresses of device memory; see include/qattn.h) -------------------
+    def rope_positions(self, n: int):
+        """RoPE tables for positions [0, n) (never shrinks; synchronises)."""
+        self._check(lib().qa_rope_positions(self._h, n))
+
+    def paged_append(self, pages: Pages, table, n_seqs, table_cols, row_seq, row_len, row_pos, n, layer, n_layers,
+                     q_pre, k_pre, v, q_out):
+        """n new rows into pages; row_seq may be 0 (row r: table row r), q_out may be 0 (not wanted)."""
+        self._check(lib().qa_paged_append(self._h, pages, table, n_seqs, table_cols, row_seq or None, row_len, row_pos,
+                                          n, layer, n_layers, q_pre, k_pre, v, q_out or None))
+
+    def paged_workspace(self, n: int, n_layers: int, max_rows: int, add_weights: bool = False) -> int:
+        out = ctypes.c_size_t()
+        st = lib().qa_paged_workspace(self._h, n, n_layers, max_rows, 1 if add_weights else 0, ctypes.byref(out))
+        if st != QA_OK:
+            raise QAttnError(st, f"paged workspace of {n} rows, {n_layers} layers, {max_rows} cache rows")
+        return out.value
+
+    def paged_attn(self, pages: Pages, table, table_cols, lengths, n, layer, n_layers, q, out, add_weights, workspace,
+                   workspace_bytes):
+        """One query row per sequence over its pages; add_weights accumulates into the pool's weights."""
+        self._check(lib().qa_paged_attn(self._h, pages, table, table_cols, lengths, n, layer, n_layers, q, out,
+                                        1 if add_weights else 0, workspace, workspace_bytes))
+
+    def paged_evict(self, pages: Pages, src_table, src_cols, dst_table, dst_cols, lengths, new_lengths, n, keep, recent,
+                    kept):
+        """Keeps the last `recent` rows and the heaviest others, `keep` in all, of every layer and head."""
+        self._check(lib().qa_paged_evict(self._h, pages, src_table, src_cols, dst_table, dst_cols, lengths, new_lengths,
+                                         n, keep, recent, kept))
 
     # -- multi-GPU ------------------------------------------------------------------------
     def comm_init(self, nranks: int, rank: int, unique_id: bytes):

@@ -241,6 +241,88 @@ int qa_project_gemm(qa_ctx* ctx, const uint16_t* w, int rows, int cols, const fl
 int qa_project_group_gemm(qa_ctx* ctx, int n_mats, const uint16_t* const* w, const int* rows, int cols,
                           const float* x, int batch, float* const* y);
 
+/* ---- Paged KV cache ------------------------------------------------------------------------
+ * The cache of a serving program that does not reserve `context` rows for every sequence: rows
+ * live in fixed-size pages of a pool, a sequence is a row of a page table, and pages are handed
+ * out as it grows (or back, after an eviction). No counterpart in the reference, whose KV is one
+ * contiguous history. The pool, the tables and the lengths are the caller's DEVICE memory in
+ * every context (io_host too), so a captured decode step replays with new lengths and tables
+ * written between replays; heads, layers, norm weights, RoPE tables, device and stream are the
+ * context's. A prompt prefilled in a slot (qa_append, qa_attn_prefill) is brought into pages by
+ * qa_paged_append of the same rows: both write the same bits.
+ *
+ * A page holds page_rows consecutive cache rows of every layer, K|V and local KV head in one
+ * block; cache row t of a sequence is row t % page_rows of page table[t / page_rows].
+ * Page ids, lengths and positions are read on the device: one outside its range is skipped
+ * (nothing is read or written through it), the results of its sequence are undefined, and the
+ * next qa_sync or host-buffer call returns QA_ERR_INVALID. Table entries past a sequence's
+ * length are not read. */
+typedef struct qa_pages {
+    uint16_t* kv;        /* [n_pages][n_layers][K|V][hkv_local][page_rows][128] FP16, 16-byte aligned */
+    float* weights;      /* [n_pages][n_layers][hkv_local][page_rows] FP32 accumulated attention
+                            weights, 16-byte aligned; NULL where no call uses them */
+    int n_pages;
+    int page_rows;       /* 16, 32, 64, 128, 256 or 512 */
+} qa_pages;
+
+#define QA_MAX_PAGED_BATCH 1024       /* sequences of one attention or eviction call */
+#define QA_MAX_PAGED_ROWS (1 << 20)   /* cache rows of one sequence, new rows of one append, RoPE positions */
+
+/* Extends the RoPE tables to positions [0, n) (at creation: the context's `context` positions;
+ * never shrinks). Rows of a paged cache may sit at any such position, since an eviction shortens
+ * a cache and not its sequence's position. Same table values as core.cpp:288 for every position.
+ * Synchronises; not allowed while the stream is capturing, and graphs captured before it must be
+ * captured again. */
+int qa_rope_positions(qa_ctx* ctx, int n);
+
+/* Fused append of n new rows to pages: the arithmetic of qa_append, bit for bit (core.cpp:395-406),
+ * with every row's place given by device arrays of n ints:
+ *   row_seq   table row of its sequence (NULL: row r belongs to table row r)
+ *   row_len   rows that its sequence holds with this one, so it becomes cache row row_len - 1;
+ *             0: a padded row, nothing is stored and its q_out row is zero
+ *   row_pos   its RoPE position, below the context's RoPE positions
+ * table: device, [n_seqs][table_cols] page ids. Rows of one call have distinct places. q_pre, k_pre,
+ * v, q_out as for qa_append, 16-byte aligned (q_out NULL: not wanted); 1 <= n <= QA_MAX_PAGED_ROWS.
+ * Prompt rows and single tokens, of any mix of sequences, go in one call. Where pages->weights is
+ * given, a new row's accumulated weights start at zero. */
+int qa_paged_append(qa_ctx* ctx, const qa_pages* pages, const int* table, int n_seqs, int table_cols,
+                    const int* row_seq, const int* row_len, const int* row_pos, int n, int layer, int n_layers,
+                    const float* q_pre, const float* k_pre, const float* v, float* q_out);
+
+/* Bytes of the workspace of qa_paged_attn calls with at most n rows, n_layers layers and
+ * max_rows = table_cols * page_rows, with or without add_weights. */
+int qa_paged_workspace(const qa_ctx* ctx, int n, int n_layers, int max_rows, int add_weights, size_t* bytes);
+
+/* Attention of one query row per sequence over its pages, split over the cache's length and
+ * joined (flash-decoding): row b attends to cache rows [0, lengths[b]) of table row b, softmax(q.k /
+ * sqrt(128)) . V in FP32, as qa_attn_decode_batch does over slots. lengths (device, n ints) count
+ * the new row once it is appended; a row of length 0 (padding) gives zeros. Rows may share pages.
+ * q, out: [n_layers][n][hq_local][128], 16-byte aligned; 1 <= n <= QA_MAX_PAGED_BATCH.
+ * add_weights != 0 also adds, for every cache row and KV head, the softmax weights of the head's
+ * query heads to pages->weights (one FP32 addition per call and row, so the results are
+ * reproducible; where rows of a call share a page, its additions come in any order).
+ * workspace: device memory of qa_paged_workspace bytes, 16-byte aligned, contents ignored; calls
+ * that may overlap on the GPU (other streams, other graphs) each need their own. */
+int qa_paged_attn(qa_ctx* ctx, const qa_pages* pages, const int* table, int table_cols, const int* lengths, int n,
+                  int layer, int n_layers, const float* q, float* out, int add_weights, void* workspace,
+                  size_t workspace_bytes);
+
+/* Eviction by accumulated attention weight: every sequence b with more than `keep` cached rows
+ * keeps, in each layer and KV head for itself, its last `recent` rows and, of the older rows, the
+ * keep - recent with the largest accumulated weights (ties: the lower row; NaN below everything).
+ * The kept rows move, in their order, with their weights, to rows [0, keep) of dst_table's row b.
+ * Sequences of at most `keep` rows keep all of them. All layers of the context.
+ *   src_table [n][src_cols], dst_table [n][dst_cols], lengths [n], new_lengths [n]: device ints.
+ * In place: dst_table names the same pages (it may be src_table itself, and new_lengths may be
+ * lengths); otherwise a sequence's dst pages are disjoint from every src page of the call. No two
+ * sequences share a dst page; in place, src pages are not shared either. new_lengths[b] =
+ * min(lengths[b], keep). kept: device, [n][n_layers][hkv_local][keep] ints, receives each kept
+ * row's old index (ascending; -1 past new_lengths[b]). Rows of dst pages past new_lengths[b] are
+ * left as they were. keep >= 1, 0 <= recent <= keep, keep <= dst_cols * page_rows;
+ * 1 <= n <= QA_MAX_PAGED_BATCH. Asynchronous on the context stream. */
+int qa_paged_evict(qa_ctx* ctx, const qa_pages* pages, const int* src_table, int src_cols, const int* dst_table,
+                   int dst_cols, const int* lengths, int* new_lengths, int n, int keep, int recent, int* kept);
+
 /* ---- Multi-GPU: KV-head sharding and prefill -> decode handoff (NCCL over NVLink) -------
  * No counterpart in the reference, a single-host CPU engine. One process per GPU; each
  * context holds KV heads [kv_head_begin, kv_head_begin + kv_head_count) with their GQA
