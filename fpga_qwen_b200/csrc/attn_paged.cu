@@ -4,27 +4,44 @@
 // group: s_t = q_h . k_t / sqrt(128), p = softmax(s), out_h = sum_t p_t v_t, all in FP32 over the
 // FP16 rows; with add_weights also weights[t] += p_t of both heads.
 //
-// Even split (stream-K style): the 16-row blocks of all (layer, row, KV head) units are laid end
-// to end and cut into equal ranges, one per CTA, whatever the lengths are; lengths are read on
-// the device, so every CTA first scans them. A range can end inside one unit and continue in the
-// next. Each warp takes every fourth block of the CTA's part of a unit (a segment) with its own
-// running maximum and sum; the CTA merges its warps at the segment's end. A unit inside one range
-// is finished there; a unit that several ranges share leaves one record (max, sum, 2 x 128
-// partial output) per range, and a second launch joins them in range order (no atomics, so the
-// result does not depend on timing). At most two units of a range are shared (its first and its
+// Bound by HBM: 512 bytes of K and V a row and KV head for 1,024 flops. What keeps HBM busy:
+//   * Even split (stream-K style). The 16-row blocks of all (layer, row, KV head) units are laid
+//     end to end and cut into equal ranges, one per CTA (2 per SM), whatever the lengths are;
+//     lengths are read on the device, so every CTA first scans them. A range can end inside one
+//     unit and continue in the next.
+//   * Every warp is its own pipeline: it takes every fourth block of the range, and one lane keeps
+//     STAGES blocks (K and V rows, 8 KB) in flight into the warp's ring with bulk copies, across
+//     unit boundaries, 192 KB per SM. A block never crosses a page, so a block is one page id; the
+//     next id is loaded one block ahead. No barrier between the warps inside a unit: each has its
+//     own running maximum and sum, merged through shared memory when the unit's part ends.
+//   * Both query heads of a KV head share its rows in registers.
+// A unit inside one range is finished there; a unit that several ranges share leaves one record
+// (max, sum, 2 x 128 partial output) per range, and a second launch, whose CTAs wait ready behind
+// the first's (programmatic dependent launch), joins them in range order: no atomics, so the
+// result does not depend on timing. At most two units of a range are shared (its first and its
 // last), so the records are 2 per CTA, whatever the batch.
 //
 // The weights need the final maximum and sum: the logits go to the workspace (8 bytes a row and
 // KV head against 512 of K and V) and become weights when the unit is finished, in this launch or
 // in the joining one. Each (row, KV head) weight gets one FP32 addition.
+//
+// Every wait is bounded: on expiry the CTA records an error code, consumes no further block, and
+// drains its copies before it exits.
 #include "qattn_common.cuh"
 #include "sm100.cuh"
 
 namespace qattn {
 namespace {
 
+using namespace sm100;
+
 constexpr int THREADS = 128, WARPS = THREADS / 32;
 constexpr int BLK = PAGED_BLK;
+constexpr int STAGES = 3;                     // blocks in flight per warp
+constexpr int HALF_STAGE = BLK * D * 2;       // K rows, then V rows of a block: 4 KB each
+constexpr int STAGE = 2 * HALF_STAGE;
+constexpr int RING = WARPS * STAGES * STAGE;
+constexpr int WAIT_CODE = 43;                 // error code of an expired wait
 constexpr int CTAS = NUM_SMS_B200 * 2;        // ranges
 constexpr int MIN_BLOCKS = 4;                 // blocks per range, at least (64 rows)
 
@@ -87,15 +104,48 @@ __device__ __forceinline__ void add_weights(const PagedAttnArgs& a, const PagedU
     }
 }
 
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
+    unsigned long long r, ua = *reinterpret_cast<unsigned long long*>(&a), ub = *reinterpret_cast<unsigned long long*>(&b),
+                          uc = *reinterpret_cast<unsigned long long*>(&c);
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(ua), "l"(ub), "l"(uc));
+    return *reinterpret_cast<float2*>(&r);
+}
+
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+// v[i] summed over the 16 lanes of each half-warp, for i = 0..15: the lane with sl == i gets sum i.
+__device__ __forceinline__ float transpose_sum16(const float (&v)[16], int sl) {
+    float w8[8], w4[4], w2[2];
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) w8[i] = (sl & 8 ? v[i + 8] : v[i]) + __shfl_xor_sync(0xffffffffu, sl & 8 ? v[i] : v[i + 8], 8);
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) w4[i] = (sl & 4 ? w8[i + 4] : w8[i]) + __shfl_xor_sync(0xffffffffu, sl & 4 ? w8[i] : w8[i + 4], 4);
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) w2[i] = (sl & 2 ? w4[i + 2] : w4[i]) + __shfl_xor_sync(0xffffffffu, sl & 2 ? w4[i] : w4[i + 2], 2);
+    return (sl & 1 ? w2[1] : w2[0]) + __shfl_xor_sync(0xffffffffu, sl & 1 ? w2[0] : w2[1], 1);
+}
+
 __global__ void __launch_bounds__(THREADS, 2) attn_paged_split_kernel(const PagedAttnArgs a) {
+    extern __shared__ __align__(128) uint8_t ring[];         // [WARPS][STAGES][K rows | V rows]
+    __shared__ __align__(8) uint64_t full[WARPS][STAGES];
     __shared__ int start[MAX_PAGED_BATCH + 1];
     __shared__ int warp_sum[WARPS];
-    __shared__ float s_stat[WARPS][4];                       // per warp: max and sum of both heads
-    __shared__ __align__(16) float s_acc[WARPS][GROUP][D];
+    __shared__ float s_stat[2][WARPS][4];                    // by segment parity: max and sum of both heads
+    __shared__ __align__(16) float s_acc[2][WARPS][GROUP][D];
+    __shared__ int abort_flag, never_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int hw = lane >> 4, sl = lane & 15;                // half-warp: rows of one parity; 8 channels a lane
     const int hq = GROUP * a.kv.hkv;
-    const PagedSplit sp = scan_lengths(a, start, warp_sum);
+    if (tid == 0) {
+        abort_flag = 0; never_abort = 0;
+        for (int i = 0; i < WARPS * STAGES; ++i) mbar_init(&full[0][0] + i, 1);
+        fence_mbar_init();
+    }
+    const PagedSplit sp = scan_lengths(a, start, warp_sum);   // its barriers publish the ring's too
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (blockIdx.x == 0)
         for (int b = tid; b < a.n; b += THREADS)
             if (a.lengths[b] != row_length(a, b)) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
@@ -110,78 +160,140 @@ __global__ void __launch_bounds__(THREADS, 2) attn_paged_split_kernel(const Page
     const long long g_begin = sp.begin(c), g_end = sp.begin(c + 1);
     const float qscale = 1.4426950408889634f * 0.08838834764831845f;   // log2(e)/sqrt(128)
     const int mask = (1 << a.kv.shift) - 1;
+    uint8_t* const my_ring = ring + warp * (STAGES * STAGE);
+    uint64_t* const my_full = full[warp];
 
+    // ---- producer side of the warp: blocks g_begin + warp, + WARPS, ... of the range ----
     PagedUnit u = paged_unit_of(start, a.n, a.kv.hkv, g_begin);
-    for (long long g = g_begin; g < g_end;) {
-        if (g != g_begin) paged_next_unit(start, a.n, a.kv.hkv, u);
-        const int blk0 = (int)(g - u.off);
+    PagedUnit pu = u;
+    long long pg = g_begin + warp;                           // next block to copy
+    uint32_t issued = 0, consumed = 0, valid = 0;            // valid: bit per stage, the block was copied
+    int next_page = -1;
+    auto find_page = [&]() {                                 // page id of block pg (loaded ahead of its use)
+        if (pg >= g_end) return;
+        while (pg >= pu.off + pu.nblk) paged_next_unit(start, a.n, a.kv.hkv, pu);
+        next_page = __ldg(a.table + (size_t)pu.b * a.cols + ((int)(pg - pu.off) * BLK >> a.kv.shift));
+    };
+    auto produce = [&]() {
+        if (pg >= g_end) return;
+        const int stage = issued % STAGES;
+        const int t0 = (int)(pg - pu.off) * BLK;
+        const uint32_t bytes = min(BLK, row_length(a, pu.b) - t0) * (D * 2);
+        const bool ok = a.kv.has(next_page);
+        valid = ok ? valid | 1u << stage : valid & ~(1u << stage);
+        if (lane == 0) {
+            if (ok) {
+                const int layer = a.layer0 + pu.l;
+                mbar_arrive_expect_tx(&my_full[stage], 2 * bytes);
+                bulk_copy(my_ring + stage * STAGE, a.kv.row(next_page, layer, 0, pu.kh, t0 & mask), bytes, &my_full[stage]);
+                bulk_copy(my_ring + stage * STAGE + HALF_STAGE, a.kv.row(next_page, layer, 1, pu.kh, t0 & mask), bytes,
+                          &my_full[stage]);
+            } else {
+                mbar_arrive(&my_full[stage]);
+                atomicCAS(a.error, 0, PAGED_BAD_PAGE);
+            }
+        }
+        ++issued;
+        pg += WARPS;
+        find_page();
+    };
+    find_page();
+    for (int i = 0; i < STAGES; ++i) produce();
+
+    auto load_q = [&](const PagedUnit& w, float4 (&x)[2 * GROUP]) {
+        const size_t row = ((size_t)w.l * a.n + w.b) * hq + (size_t)w.kh * GROUP;
+        #pragma unroll
+        for (int i = 0; i < 2 * GROUP; ++i)
+            x[i] = __ldg(reinterpret_cast<const float4*>(a.q + (row + (i >> 1)) * D + sl * 8) + (i & 1));
+    };
+    float4 q_raw[2 * GROUP];
+    load_q(u, q_raw);
+    long long my_g = g_begin + warp;                         // next block of this warp to consume
+    int parity = 0;
+    for (long long g = g_begin; g < g_end; parity ^= 1) {
         const int cnt = (int)(min(u.off + u.nblk, g_end) - g);
-        const int len = row_length(a, u.b), layer = a.layer0 + u.l;
-        const size_t qrow = ((size_t)u.l * a.n + u.b) * hq + (size_t)u.kh * GROUP;
-        float q[GROUP][8], acc[GROUP][8];
+        const int len = row_length(a, u.b);
+        float2 q[GROUP][4], acc[GROUP][4];
         #pragma unroll
         for (int i = 0; i < GROUP; ++i) {
-            const float4* src = reinterpret_cast<const float4*>(a.q + (qrow + i) * D + sl * 8);
-            const float4 x = __ldg(src), y = __ldg(src + 1);
-            q[i][0] = x.x * qscale; q[i][1] = x.y * qscale; q[i][2] = x.z * qscale; q[i][3] = x.w * qscale;
-            q[i][4] = y.x * qscale; q[i][5] = y.y * qscale; q[i][6] = y.z * qscale; q[i][7] = y.w * qscale;
+            const float4 x = q_raw[2 * i], y = q_raw[2 * i + 1];
+            q[i][0] = make_float2(x.x * qscale, x.y * qscale); q[i][1] = make_float2(x.z * qscale, x.w * qscale);
+            q[i][2] = make_float2(y.x * qscale, y.y * qscale); q[i][3] = make_float2(y.z * qscale, y.w * qscale);
             #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[i][e] = 0.f;
+            for (int e = 0; e < 4; ++e) acc[i][e] = make_float2(0.f, 0.f);
+        }
+        PagedUnit nu = u;                                    // the next segment's queries, loaded meanwhile
+        if (g + cnt < g_end) {
+            paged_next_unit(start, a.n, a.kv.hkv, nu);
+            load_q(nu, q_raw);
         }
         float m = -INFINITY, l = 0.f;                        // of head sl & 1, this lane's share of the sum
-        for (int j = warp; j < cnt; j += WARPS) {
-            const int t0 = (blk0 + j) * BLK, rows = min(BLK, len - t0);
-            const int page = a.table[(size_t)u.b * a.cols + (t0 >> a.kv.shift)];
-            if (!a.kv.has(page)) {
-                if (lane == 0) atomicCAS(a.error, 0, PAGED_BAD_PAGE);
-                continue;
-            }
-            const uint4* K = reinterpret_cast<const uint4*>(a.kv.row(page, layer, 0, u.kh, t0 & mask));
-            const uint4* V = reinterpret_cast<const uint4*>(a.kv.row(page, layer, 1, u.kh, t0 & mask));
-            // row 2i + hw of the block, head gq: this lane's 8 channels, then the sum over 16 lanes
-            float s = -INFINITY;                             // kept by the lane with sl == 2i + gq
-            #pragma unroll
-            for (int i = 0; i < BLK / 2; ++i) {
-                const int t = 2 * i + hw;
-                uint4 kr = make_uint4(0, 0, 0, 0);
-                if (t < rows) kr = K[t * 16 + sl];
-                float kf[8];
-                unpack8(kr, kf);
+        for (; my_g < g + cnt; my_g += WARPS) {
+            const int stage = consumed % STAGES;
+            bool got = mbar_wait(&my_full[stage], (consumed / STAGES) & 1, &abort_flag);
+            if (!got) { abort_flag = 1; atomicCAS(a.error, 0, WAIT_CODE); }
+            got = __all_sync(0xffffffffu, got);
+            const uint8_t* buf = my_ring + stage * STAGE;
+            const int rows = min(BLK, len - (int)(my_g - u.off) * BLK);
+            if (got && (valid >> stage & 1)) {
+                // row 2i + hw of the block and head gq: partial sums over this lane's 8 channels, then
+                // over the 16 lanes; the lane with sl == 2i + gq keeps the logit
+                float v[16];
                 #pragma unroll
-                for (int gq = 0; gq < GROUP; ++gq) {
-                    float d = 0.f;
+                for (int i = 0; i < BLK / 2; ++i) {
+                    float kf[8];
+                    unpack8(*reinterpret_cast<const uint4*>(buf + (2 * i + hw) * (D * 2) + sl * 16), kf);
                     #pragma unroll
-                    for (int e = 0; e < 8; ++e) d = fmaf(q[gq][e], kf[e], d);
+                    for (int gq = 0; gq < GROUP; ++gq) {
+                        float2 d = make_float2(0.f, 0.f);
+                        #pragma unroll
+                        for (int e = 0; e < 4; ++e) d = ffma2(q[gq][e], make_float2(kf[2 * e], kf[2 * e + 1]), d);
+                        v[2 * i + gq] = d.x + d.y;
+                    }
+                }
+                const int t = 2 * (sl >> 1) + hw;            // this lane's row of the block
+                const bool there = t < rows;
+                float s = transpose_sum16(v, sl);
+                if (!there) s = -INFINITY;                   // (stale bytes of the ring)
+                if (a.add_weights) a.logits[my_g * (BLK * 2) + t * 2 + (sl & 1)] = s;
+                float mb = s;
+                #pragma unroll
+                for (int o = 2; o <= 16; o <<= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+                if (__any_sync(0xffffffffu, mb > m)) {
+                    const float mn = fmaxf(m, mb);
+                    const float scale = exp2_from(m, mn);
+                    m = mn;
+                    l *= scale;
+                    const float other = __shfl_xor_sync(0xffffffffu, scale, 1);
+                    const float sc0 = sl & 1 ? other : scale, sc1 = sl & 1 ? scale : other;
                     #pragma unroll
-                    for (int o = 8; o >= 1; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-                    if (sl == 2 * i + gq && t < rows) s = d;
+                    for (int e = 0; e < 4; ++e) {
+                        acc[0][e].x *= sc0; acc[0][e].y *= sc0;
+                        acc[1][e].x *= sc1; acc[1][e].y *= sc1;
+                    }
+                }
+                const float p = there ? exp2_from(s, m) : 0.f;
+                l += p;
+                #pragma unroll
+                for (int i = 0; i < BLK / 2; ++i) {
+                    uint4 vr = *reinterpret_cast<const uint4*>(buf + HALF_STAGE + (2 * i + hw) * (D * 2) + sl * 16);
+                    if (2 * i + hw >= rows) vr = make_uint4(0, 0, 0, 0);   // stale bytes count nothing, whatever they are
+                    float vf[8];
+                    unpack8(vr, vf);
+                    const float p0 = __shfl_sync(0xffffffffu, p, (lane & 16) + 2 * i);
+                    const float p1 = __shfl_sync(0xffffffffu, p, (lane & 16) + 2 * i + 1);
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 v2 = make_float2(vf[2 * e], vf[2 * e + 1]);
+                        acc[0][e] = ffma2(make_float2(p0, p0), v2, acc[0][e]);
+                        acc[1][e] = ffma2(make_float2(p1, p1), v2, acc[1][e]);
+                    }
                 }
             }
-            if (a.add_weights) a.logits[(g + j) * (BLK * 2) + (2 * (sl >> 1) + hw) * 2 + (sl & 1)] = s;
-            float mb = s;
-            #pragma unroll
-            for (int o = 2; o <= 16; o <<= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
-            const float mn = fmaxf(m, mb);
-            const float scale = exp2_from(m, mn);
-            const bool there = 2 * (sl >> 1) + hw < rows;
-            const float p = there ? exp2_from(s, mn) : 0.f;
-            m = mn;
-            l = l * scale + p;
-            const float other = __shfl_xor_sync(0xffffffffu, scale, 1);
-            const float sc0 = sl & 1 ? other : scale, sc1 = sl & 1 ? scale : other;
-            #pragma unroll
-            for (int e = 0; e < 8; ++e) { acc[0][e] *= sc0; acc[1][e] *= sc1; }
-            #pragma unroll
-            for (int i = 0; i < BLK / 2; ++i) {
-                const int t = 2 * i + hw;
-                uint4 vr = make_uint4(0, 0, 0, 0);           // rows past the length count nothing, whatever they hold
-                if (t < rows) vr = V[t * 16 + sl];
-                float vf[8];
-                unpack8(vr, vf);
-                const float p0 = __shfl_sync(0xffffffffu, p, (lane & 16) + 2 * i);
-                const float p1 = __shfl_sync(0xffffffffu, p, (lane & 16) + 2 * i + 1);
-                #pragma unroll
-                for (int e = 0; e < 8; ++e) { acc[0][e] = fmaf(p0, vf[e], acc[0][e]); acc[1][e] = fmaf(p1, vf[e], acc[1][e]); }
+            __syncwarp();                                    // the stage is read by all lanes
+            if (got) {
+                ++consumed;
+                produce();
             }
         }
         // ---- merge the warps ----
@@ -190,25 +302,29 @@ __global__ void __launch_bounds__(THREADS, 2) attn_paged_split_kernel(const Page
         #pragma unroll
         for (int i = 0; i < GROUP; ++i)
             #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                acc[i][e] += __shfl_xor_sync(0xffffffffu, acc[i][e], 16);
-                if (hw == 0) s_acc[warp][i][sl * 8 + e] = acc[i][e];
+            for (int e = 0; e < 4; ++e) {
+                acc[i][e].x += __shfl_xor_sync(0xffffffffu, acc[i][e].x, 16);
+                acc[i][e].y += __shfl_xor_sync(0xffffffffu, acc[i][e].y, 16);
+                if (hw == 0) *reinterpret_cast<float2*>(&s_acc[parity][warp][i][sl * 8 + 2 * e]) = acc[i][e];
             }
-        if (lane < 2) { s_stat[warp][lane] = m; s_stat[warp][2 + lane] = l; }
-        __syncthreads();
+        if (lane < 2) { s_stat[parity][warp][lane] = m; s_stat[parity][warp][2 + lane] = l; }
+        __syncthreads();                                     // (the other parity's buffers were read before it)
         float M[GROUP], L[GROUP], o[GROUP];
         #pragma unroll
         for (int i = 0; i < GROUP; ++i) {
-            M[i] = s_stat[0][i];
-            for (int w = 1; w < WARPS; ++w) M[i] = fmaxf(M[i], s_stat[w][i]);
+            M[i] = s_stat[parity][0][i];
+            #pragma unroll
+            for (int w = 1; w < WARPS; ++w) M[i] = fmaxf(M[i], s_stat[parity][w][i]);
             L[i] = 0.f; o[i] = 0.f;
+            #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
-                const float f = exp2_from(s_stat[w][i], M[i]);
-                L[i] += f * s_stat[w][2 + i];
-                o[i] += f * s_acc[w][i][tid];
+                const float f = exp2_from(s_stat[parity][w][i], M[i]);
+                L[i] += f * s_stat[parity][w][2 + i];
+                o[i] += f * s_acc[parity][w][i][tid];
             }
         }
         if (cnt == u.nblk) {
+            const size_t qrow = ((size_t)u.l * a.n + u.b) * hq + (size_t)u.kh * GROUP;
             #pragma unroll
             for (int i = 0; i < GROUP; ++i) a.out[(qrow + i) * D + tid] = o[i] / L[i];
             if (a.add_weights) add_weights(a, u, g, cnt, M, L);
@@ -219,8 +335,10 @@ __global__ void __launch_bounds__(THREADS, 2) attn_paged_split_kernel(const Page
             for (int i = 0; i < GROUP; ++i) rec[4 + i * D + tid] = o[i];
         }
         g += cnt;
-        __syncthreads();                                     // s_acc, s_stat and the logits are read
+        u = nu;
     }
+    // drain: copies issued but not consumed (after an expired wait) must land before the CTA exits
+    for (; consumed < issued; ++consumed) mbar_wait(&my_full[consumed % STAGES], (consumed / STAGES) & 1, &never_abort, 500000000ull);
 }
 
 // CTA c joins the unit whose first range is c, and adds the weights of the parts of shared units
@@ -228,8 +346,11 @@ __global__ void __launch_bounds__(THREADS, 2) attn_paged_split_kernel(const Page
 __global__ void __launch_bounds__(THREADS) attn_paged_join_kernel(const PagedAttnArgs a) {
     __shared__ int start[MAX_PAGED_BATCH + 1];
     __shared__ int warp_sum[WARPS];
-    const int tid = threadIdx.x, c = blockIdx.x, hq = GROUP * a.kv.hkv;
+    __shared__ float s_f[CTAS][GROUP];                       // factor of each record
+    __shared__ float red[2 * GROUP][WARPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x, hq = GROUP * a.kv.hkv;
     const PagedSplit sp = scan_lengths(a, start, warp_sum);
+    asm volatile("griddepcontrol.wait;" ::: "memory");       // the split launch is complete and its stores visible
     if (sp.total == 0 || c >= sp.ctas) return;
     const long long g_begin = sp.begin(c), g_end = sp.begin(c + 1);
     long long done = -1;
@@ -237,24 +358,60 @@ __global__ void __launch_bounds__(THREADS) attn_paged_join_kernel(const PagedAtt
         const PagedUnit u = paged_unit_of(start, a.n, a.kv.hkv, side ? g_end - 1 : g_begin);
         if (u.off == done) continue;
         done = u.off;
-        const int c_first = sp.range_of(u.off), c_last = sp.range_of(u.off + u.nblk - 1);
-        if (c_first == c_last || (c != c_first && !a.add_weights)) continue;
-        float M[GROUP] = {-INFINITY, -INFINITY}, L[GROUP] = {0.f, 0.f}, o[GROUP] = {0.f, 0.f};
-        for (int r = c_first; r <= c_last; ++r) {
-            const float* rec = a.records + ((size_t)r * 2 + (r == c_first && u.off != sp.begin(r))) * PARTIAL_FLOATS;
+        const int c_first = sp.range_of(u.off), c_last = sp.range_of(u.off + u.nblk - 1), nrec = c_last - c_first + 1;
+        if (nrec == 1 || (c != c_first && !a.add_weights)) continue;
+        // record i of the unit: range c_first + i; slot 0 but in the first range, unless it begins the range
+        const float* first = a.records + ((size_t)c_first * 2 + (u.off != sp.begin(c_first))) * PARTIAL_FLOATS;
+        const float* others = a.records + (size_t)c_first * 2 * PARTIAL_FLOATS;
+        float M[GROUP] = {-INFINITY, -INFINITY}, L[GROUP] = {0.f, 0.f};
+        __syncthreads();                                     // s_f and red are free
+        for (int i = tid; i < nrec; i += THREADS) {
+            const float4 st = *reinterpret_cast<const float4*>(i ? others + (size_t)i * 2 * PARTIAL_FLOATS : first);
+            M[0] = fmaxf(M[0], st.x); M[1] = fmaxf(M[1], st.y);
+        }
+        #pragma unroll
+        for (int k = 0; k < GROUP; ++k) {
             #pragma unroll
-            for (int i = 0; i < GROUP; ++i) {
-                const float mn = fmaxf(M[i], rec[i]);
-                const float f = exp2_from(M[i], mn), fr = exp2_from(rec[i], mn);
-                M[i] = mn;
-                L[i] = L[i] * f + rec[GROUP + i] * fr;
-                o[i] = o[i] * f + rec[4 + i * D + tid] * fr;
-            }
+            for (int x = 16; x >= 1; x >>= 1) M[k] = fmaxf(M[k], __shfl_xor_sync(0xffffffffu, M[k], x));
+            if (lane == 0) red[k][warp] = M[k];
+        }
+        __syncthreads();
+        #pragma unroll
+        for (int k = 0; k < GROUP; ++k)
+            #pragma unroll
+            for (int w = 0; w < WARPS; ++w) M[k] = fmaxf(M[k], red[k][w]);
+        for (int i = tid; i < nrec; i += THREADS) {
+            const float4 st = *reinterpret_cast<const float4*>(i ? others + (size_t)i * 2 * PARTIAL_FLOATS : first);
+            const float f0 = exp2_from(st.x, M[0]), f1 = exp2_from(st.y, M[1]);
+            s_f[i][0] = f0; s_f[i][1] = f1;
+            L[0] += f0 * st.z; L[1] += f1 * st.w;
+        }
+        #pragma unroll
+        for (int k = 0; k < GROUP; ++k) {
+            #pragma unroll
+            for (int x = 16; x >= 1; x >>= 1) L[k] += __shfl_xor_sync(0xffffffffu, L[k], x);
+            if (lane == 0) red[GROUP + k][warp] = L[k];
+        }
+        __syncthreads();
+        #pragma unroll
+        for (int k = 0; k < GROUP; ++k) {
+            L[k] = 0.f;
+            #pragma unroll
+            for (int w = 0; w < WARPS; ++w) L[k] += red[GROUP + k][w];
         }
         if (c == c_first) {
+            float o[GROUP];
+            #pragma unroll
+            for (int k = 0; k < GROUP; ++k) o[k] = s_f[0][k] * first[4 + k * D + tid];
+            #pragma unroll 8
+            for (int i = 1; i < nrec; ++i) {
+                const float* rec = others + (size_t)i * 2 * PARTIAL_FLOATS + 4 + tid;
+                #pragma unroll
+                for (int k = 0; k < GROUP; ++k) o[k] += s_f[i][k] * rec[k * D];
+            }
             const size_t qrow = ((size_t)u.l * a.n + u.b) * hq + (size_t)u.kh * GROUP;
             #pragma unroll
-            for (int i = 0; i < GROUP; ++i) a.out[(qrow + i) * D + tid] = o[i] / L[i];
+            for (int k = 0; k < GROUP; ++k) a.out[(qrow + k) * D + tid] = o[k] / L[k];
         }
         if (a.add_weights) {
             const long long g = max(u.off, g_begin);
@@ -273,9 +430,16 @@ size_t paged_attn_workspace(int n, int n_layers, int hkv, int max_rows, bool wei
 }
 
 cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
-    attn_paged_split_kernel<<<CTAS, THREADS, 0, s>>>(a);
-    attn_paged_join_kernel<<<CTAS, THREADS, 0, s>>>(a);
-    return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(attn_paged_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING);
+    if (e != cudaSuccess) return e;
+    attn_paged_split_kernel<<<CTAS, THREADS, RING, s>>>(a);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(CTAS); cfg.blockDim = dim3(THREADS); cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel, a);
 }
 
 }  // namespace qattn
