@@ -72,7 +72,8 @@ __global__ void __launch_bounds__(TPB * 4 * HKV) kv_append_kernel(const AppendAr
         const int kind = r < HQ ? 0 : (r < HQ + HKV ? 1 : 2);
         if (tb < ntok && kind < 2) {
             const float* slot = &slots[tb * SLOT];
-            norm_rope_row(&tile[row * STRIDE], slot + 128 + kind * D, slot, slot + 64, a.eps);
+            float* x = &tile[row * STRIDE];
+            norm_rope_row(x, slot + 128 + kind * D, slot, slot + 64, rms_inv(x, a.eps));
         }
     }
     __syncthreads();

@@ -6,10 +6,12 @@
 // padding: nothing is stored and its query rows are zero. Places outside their tables are
 // recorded in the error block and skipped.
 //
-// Layout as in kv_append.cu: a block owns TPB tokens of one layer, one thread per head row; rows,
-// RoPE rows and norm weights are staged in shared memory with 16-byte cp.async copies, the
-// sequential FP64 sum of squares runs one row per thread, and the stores are coalesced. The
-// table look-up (row_len -> page id) runs on one thread per token while the copies are in flight.
+// Layout as in kv_append.cu: a block owns TPB tokens of one layer, one thread per head row (one
+// warp); rows are staged in shared memory with 16-byte cp.async copies, the sequential FP64 sum of
+// squares runs one row per thread, and the stores are coalesced. Two chains of dependent loads hang
+// on the row arrays, position -> RoPE rows and length -> table -> page id; both stay off the
+// critical path: the RoPE rows are a second copy group, needed only once the sums are done, and
+// the page ids stay in registers that the stores are the first to read.
 // HBM-bound: 28,672 algorithmic bytes per (token, layer) at 8 KV heads.
 #include "norm_rope.cuh"
 
@@ -26,75 +28,87 @@ __device__ __forceinline__ void cp_async16(void* smem, const void* gmem) {
 
 template <int HKV, int TPB>
 __global__ void __launch_bounds__(TPB * 4 * HKV) kv_paged_append_kernel(const PagedAppendArgs a) {
-    constexpr int HQ = GROUP * HKV, R = HQ + 2 * HKV, ROWS = TPB * R, WARPS = (ROWS + 31) / 32;
+    constexpr int HQ = GROUP * HKV, R = HQ + 2 * HKV, ROWS = TPB * R;
+    static_assert(ROWS == 32, "one warp: the page ids travel by shuffle");
     extern __shared__ __align__(16) float smem[];
     float* tile = smem;                                   // [ROWS][STRIDE]
     float* slots = smem + ROWS * STRIDE;                  // [TPB][SLOT]
-    __shared__ int s_page[TPB], s_row[TPB];               // page < 0: nothing to store
     const int l = blockIdx.y, layer = a.layer0 + l;
     const int b0 = blockIdx.x * TPB;
     const int ntok = min(TPB, a.n - b0);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x;
     const size_t tok_base = (size_t)l * a.n + b0;
     const int r_first = a.q_out ? 0 : HQ;                 // without q_out the query rows are not touched
 
-    for (int row = warp; row < ntok * R; row += WARPS) {
+    // lane tb < ntok: the place of token b0 + tb
+    int pos = 0, len = 0, seq = 0;
+    if (lane < ntok) {
+        pos = __ldg(a.row_pos + b0 + lane);
+        len = __ldg(a.row_len + b0 + lane);
+        seq = a.row_seq ? __ldg(a.row_seq + b0 + lane) : b0 + lane;
+    }
+    #pragma unroll 8
+    for (int row = 0; row < ROWS; ++row) {
         const int tb = row / R, r = row - tb * R;
-        if (r < r_first) continue;
+        if (r < r_first || tb >= ntok) continue;
         const size_t tok = tok_base + tb;
         const float* src = r < HQ ? a.q_pre + (tok * HQ + r) * D
                          : r < HQ + HKV ? a.k_pre + (tok * HKV + (r - HQ)) * D
                                         : a.v_pre + (tok * HKV + (r - HQ - HKV)) * D;
         cp_async16(&tile[row * STRIDE + lane * 4], src + lane * 4);
     }
-    for (int i = threadIdx.x; i < ntok * (SLOT / 4); i += ROWS) {
-        const int tb = i / (SLOT / 4), c = i - tb * (SLOT / 4);   // 96 chunks of 16 bytes per token
-        int pos = a.row_pos[b0 + tb];
-        if ((unsigned)pos >= (unsigned)a.rope_rows) pos = 0;      // recorded and skipped below
-        const float* src = c < 16 ? a.cosines + (size_t)pos * 64 + c * 4
-                         : c < 32 ? a.sines + (size_t)pos * 64 + (c - 16) * 4
-                                  : a.norms + (size_t)layer * 2 * D + (c - 32) * 4;
-        cp_async16(&slots[tb * SLOT + c * 4], src);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    #pragma unroll
+    for (int tb = 0; tb < TPB; ++tb) {                    // 96 chunks of 16 bytes per token
+        if (tb >= ntok) break;
+        int p = __shfl_sync(0xffffffffu, pos, tb);
+        if ((unsigned)p >= (unsigned)a.rope_rows) p = 0;  // recorded and skipped below
+        cp_async16(&slots[tb * SLOT + lane * 4], lane < 16 ? a.cosines + (size_t)p * 64 + lane * 4
+                                                           : a.sines + (size_t)p * 64 + (lane - 16) * 4);
+        #pragma unroll
+        for (int c = 0; c < 2; ++c)
+            cp_async16(&slots[tb * SLOT + 128 + c * D + lane * 4], a.norms + ((size_t)layer * 2 + c) * D + lane * 4);
     }
-    if (threadIdx.x < ntok) {
-        const int b = b0 + threadIdx.x;
-        const int len = a.row_len[b], seq = a.row_seq ? a.row_seq[b] : b;
-        int code;
-        const int page = paged_place(len, seq, a.row_pos[b], a.n_seqs, a.cols, a.kv.shift, a.rope_rows, a.kv.n_pages,
-                                     a.table, &code);
-        if (code) atomicCAS(a.error, 0, code);
-        s_page[threadIdx.x] = page;
-        s_row[threadIdx.x] = (int)(((unsigned)len - 1u) & ((1u << a.kv.shift) - 1u));
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    int code = 0, page = -1;
+    if (lane < ntok)
+        page = paged_place(len, seq, pos, a.n_seqs, a.cols, a.kv.shift, a.rope_rows, a.kv.n_pages, a.table, &code);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
 
     {
-        const int row = threadIdx.x;
-        const int tb = row / R, r = row - tb * R;
-        if (tb < ntok && r >= r_first && r < HQ + HKV) {
+        const int tb = lane / R, r = lane - tb * R;
+        const bool turn = tb < ntok && r >= r_first && r < HQ + HKV;
+        float* x = &tile[lane * STRIDE];
+        const float inv = turn ? rms_inv(x, a.eps) : 0.f;
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+        if (turn) {
             const float* slot = &slots[tb * SLOT];
-            norm_rope_row(&tile[row * STRIDE], slot + 128 + (r < HQ ? 0 : D), slot, slot + 64, a.eps);
+            norm_rope_row(x, slot + 128 + (r < HQ ? 0 : D), slot, slot + 64, inv);
         }
     }
-    __syncthreads();
+    __syncwarp();
 
-    for (int row = warp; row < ntok * R; row += WARPS) {
+    if (code) atomicCAS(a.error, 0, code);
+    const int at = (int)(((unsigned)len - 1u) & ((1u << a.kv.shift) - 1u));
+    #pragma unroll 4
+    for (int row = 0; row < ROWS; ++row) {
         const int tb = row / R, r = row - tb * R;
-        if (r < r_first) continue;
+        if (r < r_first || tb >= ntok) continue;
         const float* x = &tile[row * STRIDE];
-        const int page = s_page[tb];
+        const int pg = __shfl_sync(0xffffffffu, page, tb), t = __shfl_sync(0xffffffffu, at, tb);
         if (r < HQ) {
             float* dst = a.q_out + ((tok_base + tb) * HQ + r) * D;
             reinterpret_cast<float4*>(dst)[lane] =
-                page < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(x + lane * 4);
-        } else if (page >= 0) {
+                pg < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(x + lane * 4);
+        } else if (pg >= 0) {
             const int kind = r < HQ + HKV ? 0 : 1;
             const int head = r - HQ - kind * HKV;
             if (lane < 16)
-                reinterpret_cast<uint4*>(a.kv.row(page, layer, kind, head, s_row[tb]))[lane] = half8_rn(x + lane * 8);
+                reinterpret_cast<uint4*>(a.kv.row(pg, layer, kind, head, t))[lane] = half8_rn(x + lane * 8);
             else if (lane == 16 && kind == 0 && a.kv.weights)
-                *a.kv.weight(page, layer, head, s_row[tb]) = 0.f;
+                *a.kv.weight(pg, layer, head, t) = 0.f;
         }
     }
 }

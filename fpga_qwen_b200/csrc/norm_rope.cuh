@@ -38,10 +38,9 @@ __device__ __forceinline__ void norm_rope_pair(float xa, float xb, float wa, flo
     rb = __fadd_rn(__fmul_rn(nb, c), __fmul_rn(na, s));
 }
 
-// One staged row x[0..127] in place: norm with weights w, rotation by cs[64], sn[64] (16-byte
-// aligned shared memory).
-__device__ __forceinline__ void norm_rope_row(float* x, const float* w, const float* cs, const float* sn, float eps) {
-    const float inv = rms_inv(x, eps);
+// One staged row x[0..127] in place: norm with inv and weights w, rotation by cs[64], sn[64]
+// (16-byte aligned shared memory).
+__device__ __forceinline__ void norm_rope_row(float* x, const float* w, const float* cs, const float* sn, float inv) {
     #pragma unroll 4
     for (int j = 0; j < 64; j += 4) {
         const float4 xa = *reinterpret_cast<const float4*>(x + j);
