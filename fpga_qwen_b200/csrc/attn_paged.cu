@@ -6,24 +6,40 @@
 //
 // Bound by HBM: 512 bytes of K and V a row and KV head for 1,024 flops. What keeps HBM busy:
 //   * Even split (stream-K style). The 16-row blocks of all (layer, row, KV head) units are laid
-//     end to end and cut into equal ranges, one per CTA (2 per SM), whatever the lengths are;
-//     lengths are read on the device, so every CTA first scans them. A range can end inside one
-//     unit and continue in the next.
-//   * Every warp is its own pipeline: it takes every fourth block of the range, and one lane keeps
-//     STAGES blocks (K and V rows, 8 KB) in flight into the warp's ring with bulk copies, across
-//     unit boundaries, 192 KB per SM. A block never crosses a page, so a block is one page id; the
-//     next id is loaded one block ahead. No barrier between the warps inside a unit: each has its
-//     own running maximum and sum, merged through shared memory when the unit's part ends.
-//   * Both query heads of a KV head share its rows in registers.
-// A unit inside one range is finished there; a unit that several ranges share leaves one record
-// (max, sum, 2 x 128 partial output) per range, and a second launch, whose CTAs wait ready behind
-// the first's (programmatic dependent launch), joins them in range order: no atomics, so the
-// result does not depend on timing. At most two units of a range are shared (its first and its
-// last), so the records are 2 per CTA, whatever the batch.
+//     end to end and cut into equal ranges, one per CTA (one CTA per SM), and a CTA's range again
+//     into one part per warp, whatever the lengths are; lengths are read on the device, so every
+//     CTA first scans them. A part can end inside one unit and continue in the next.
+//   * Every warp is its own pipeline from its first block to its last: one lane keeps STAGES blocks
+//     (K and V rows, 8 KB) in flight into the warp's ring with TMA copies (128-byte swizzle),
+//     across unit boundaries, 192 KB per SM. A block never crosses a page, so a block is one page
+//     id; the next id is loaded one block ahead. No barrier between the warps until all are
+//     done: a unit inside a warp's part is finished by the warp alone.
+//   * Few instructions per block. With FP32 FMAs a block of 16 rows took about 560 warp
+//     instructions (conversions, products, the sum over lanes), about what HBM leaves time for;
+//     mma.sync takes K and V as they are and needs a quarter. Both GQA heads share the tile:
+//     its N = 8 columns are the FP16 halves (high, low) of both heads' queries, or of both heads'
+//     softmax weights, twice. (A tcgen05 tile would hold 128 rows against 16 here and bring TMEM
+//     round trips, for no more bytes.)
+//
+// Numerics: FP16 rows are exact operands. A query (scaled by a power of two so that its largest
+// channel lies in [2^13, 2^14)) and a weight (exp2 of the distance to the maximum, plus 14) are
+// each the sum of two FP16 halves: 22 bits, or 2^-38 of the largest, whichever is coarser; sums are
+// FP32. The high half is rounded towards zero and neither half of a nonzero value is zero, so
+// both have its sign and an infinite key or value gives what the formula gives.
+//
+// A unit that several warps of a CTA share is merged through shared memory at the CTA's end; a
+// unit that several CTAs share leaves one record (max, sum, 2 x 128 partial output) per CTA, and a
+// second launch, whose CTAs start behind the first's (programmatic dependent launch), joins
+// them in range order: no atomics and no flags, so the result does not depend on timing and the
+// workspace needs no initial state. At most two units of a range are shared with other ranges (its
+// first and its last), so the records are 2 per CTA, whatever the batch. (Joining in the first
+// launch, by the CTA that sees all records of a unit stored, measured slower: its fences and the
+// late joins cost 8 us of 81 at 28 layers x 3970 rows.)
 //
 // The weights need the final maximum and sum: the logits go to the workspace (8 bytes a row and
-// KV head against 512 of K and V) and become weights when the unit is finished, in this launch or
-// in the joining one. Each (row, KV head) weight gets one FP32 addition.
+// KV head against 512 of K and V) and become weights when the unit is finished, by the warp, the
+// CTA or, for units shared between CTAs, in the joining launch, each CTA those of its own range.
+// Each (row, KV head) weight gets one FP32 addition.
 //
 // Every wait is bounded: on expiry the CTA records an error code, consumes no further block, and
 // drains its copies before it exits.
@@ -35,22 +51,39 @@ namespace {
 
 using namespace sm100;
 
-constexpr int THREADS = 128, WARPS = THREADS / 32;
+constexpr int WARPS = 8, THREADS = WARPS * 32;
 constexpr int BLK = PAGED_BLK;
 constexpr int STAGES = 3;                     // blocks in flight per warp
-constexpr int HALF_STAGE = BLK * D * 2;       // K rows, then V rows of a block: 4 KB each
+constexpr int HALF_STAGE = BLK * D * 2;       // K rows, then V rows of a block: 4 KB each, [channel half][row][64]
 constexpr int STAGE = 2 * HALF_STAGE;
 constexpr int RING = WARPS * STAGES * STAGE;
+constexpr int Q_WORDS = GROUP * D;            // a warp's query halves, packed (high, low)
+constexpr int CTAS = NUM_SMS_B200;            // ranges
+constexpr int MIN_BLOCKS = WARPS;             // blocks per range, at least
+constexpr int JOIN_THREADS = 256, JOIN_GROUPS = JOIN_THREADS / (GROUP * D / 4);
 constexpr int WAIT_CODE = 43;                 // error code of an expired wait
-constexpr int CTAS = NUM_SMS_B200 * 2;        // ranges
-constexpr int MIN_BLOCKS = 4;                 // blocks per range, at least (64 rows)
+
+// A part of a unit that its worker does not finish alone.
+struct Part {
+    int unit;                                 // (l * n + b) * hkv + kh, or -1: none
+    int blk0, cnt, nblk;                      // blocks [blk0, blk0 + cnt) of the unit's nblk
+    float m[GROUP], l[GROUP];
+};
+// The joining launch's view of a range's part of a shared unit.
+struct __align__(16) Shared {
+    int nrec, first, first_slot, unit;        // records of the unit (0: no such part), their first range and its slot
+    int blk0, cnt;
+    long long g;                              // its first block in the call
+};
+__device__ __forceinline__ Shared* shared_of(const PagedAttnArgs& a) { return static_cast<Shared*>(a.shared); }
 
 __device__ __forceinline__ int row_length(const PagedAttnArgs& a, int b) {
     return paged_length(a.lengths[b], a.cols, a.kv.shift);
 }
 
-// start[b] = blocks of rows [0, b); called by all threads of the CTA, n <= MAX_PAGED_BATCH.
-__device__ PagedSplit scan_lengths(const PagedAttnArgs& a, int* start, int* warp_sum) {
+// start[b] = blocks of rows [0, b), length[b] its cached rows; called by all threads of the CTA,
+// n <= MAX_PAGED_BATCH.
+__device__ __forceinline__ PagedSplit scan_lengths(const PagedAttnArgs& a, int* start, int* length, int* warp_sum) {
     constexpr int PER = MAX_PAGED_BATCH / THREADS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int v[PER], sum = 0;
@@ -58,7 +91,11 @@ __device__ PagedSplit scan_lengths(const PagedAttnArgs& a, int* start, int* warp
     for (int i = 0; i < PER; ++i) {
         const int b = tid * PER + i;
         v[i] = sum;
-        if (b < a.n) sum += (row_length(a, b) + BLK - 1) / BLK;
+        if (b < a.n) {
+            const int len = row_length(a, b);
+            length[b] = len;
+            sum += (len + BLK - 1) / BLK;
+        }
     }
     int incl = sum;
     #pragma unroll
@@ -69,7 +106,8 @@ __device__ PagedSplit scan_lengths(const PagedAttnArgs& a, int* start, int* warp
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
     int base = incl - sum;
-    for (int w = 0; w < warp; ++w) base += warp_sum[w];
+    #pragma unroll
+    for (int w = 0; w < WARPS; ++w) base += w < warp ? warp_sum[w] : 0;
     #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int b = tid * PER + i;
@@ -80,361 +118,454 @@ __device__ PagedSplit scan_lengths(const PagedAttnArgs& a, int* start, int* warp
     return paged_split((long long)a.n_layers * a.kv.hkv * start[a.n], CTAS, MIN_BLOCKS);
 }
 
-__device__ __forceinline__ void unpack8(const uint4 u, float f[8]) {
-    const __half2* h = reinterpret_cast<const __half2*>(&u);
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) { const float2 t = __half22float2(h[i]); f[2 * i] = t.x; f[2 * i + 1] = t.y; }
-}
-
 // exp2(x - m) where m is a maximum that may still be -inf (nothing seen, or only -inf logits).
 __device__ __forceinline__ float exp2_from(float x, float m) { return exp2f(x - (m == -INFINITY ? 0.f : m)); }
 
-// weights += p for the rows of blocks [g, g + cnt) of unit u, by all threads of the CTA.
-__device__ __forceinline__ void add_weights(const PagedAttnArgs& a, const PagedUnit& u, long long g, int cnt, const float M[2],
-                                            const float L[2]) {
-    const int t0 = (int)(g - u.off) * BLK, len = row_length(a, u.b);
-    const int t1 = min(t0 + cnt * BLK, len);
-    const float* s = a.logits + g * (BLK * 2);
-    for (int t = t0 + (int)threadIdx.x; t < t1; t += THREADS) {
-        const float2 x = *reinterpret_cast<const float2*>(s + (size_t)(t - t0) * 2);
-        const int page = a.table[(size_t)u.b * a.cols + (t >> a.kv.shift)];
-        if (a.kv.has(page))
-            atomicAdd(a.kv.weight(page, a.layer0 + u.l, u.kh, t & ((1 << a.kv.shift) - 1)),
-                      exp2_from(x.x, M[0]) / L[0] + exp2_from(x.y, M[1]) / L[1]);
+// weights += p for the rows of blocks [blk0, blk0 + cnt) of a unit of len rows, whose logits begin
+// at block g, by threads t of nt, four rows a thread: a vector reduction, which leaves L2 to do the
+// addition.
+__device__ __forceinline__ void add_weights(const PagedAttnArgs& a, int l, int b, int kh, int len, int blk0, int cnt, long long g,
+                                            const float (&M)[GROUP], const float (&L)[GROUP], int t, int nt) {
+    const int t0 = blk0 * BLK, rows = min(cnt * BLK, len - t0);
+    const float4* s = reinterpret_cast<const float4*>(a.logits + g * (BLK * 2));
+    const int* table = a.table + (size_t)b * a.cols;
+    const float r0 = 1.f / L[0], r1 = 1.f / L[1];
+    #pragma unroll 4
+    for (int i = t * 4; i < rows; i += nt * 4) {
+        const float4 x = s[i >> 1], y = s[(i >> 1) + 1];
+        const int page = table[(t0 + i) >> a.kv.shift];
+        const float w[4] = {exp2_from(x.x, M[0]) * r0 + exp2_from(x.y, M[1]) * r1, exp2_from(x.z, M[0]) * r0 + exp2_from(x.w, M[1]) * r1,
+                            exp2_from(y.x, M[0]) * r0 + exp2_from(y.y, M[1]) * r1, exp2_from(y.z, M[0]) * r0 + exp2_from(y.w, M[1]) * r1};
+        if (!a.kv.has(page)) continue;
+        float* dst = a.kv.weight(page, a.layer0 + l, kh, (t0 + i) & ((1 << a.kv.shift) - 1));
+        if (i + 4 <= rows)
+            asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};"
+                         ::"l"(dst), "f"(w[0]), "f"(w[1]), "f"(w[2]), "f"(w[3]) : "memory");
+        else
+            for (int k = 0; k < rows - i; ++k) atomicAdd(dst + k, w[k]);
     }
 }
 
-__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
-    unsigned long long r, ua = *reinterpret_cast<unsigned long long*>(&a), ub = *reinterpret_cast<unsigned long long*>(&b),
-                          uc = *reinterpret_cast<unsigned long long*>(&c);
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(ua), "l"(ub), "l"(uc));
-    return *reinterpret_cast<float2*>(&r);
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// d[16 x 8] += a[16 x 16] b[16 x 8], FP16 operands, FP32 sums.
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+// x, |x| < 65504, as high + low FP16 halves (high in the low 16 bits). High is x towards zero; the
+// halves of a nonzero x are nonzero and have its sign (the smallest subnormal, 2^-24, where they
+// would be zero); infinities and NaN stay in the high half.
+__device__ __forceinline__ uint32_t split_half(float x) {
+    const uint32_t tiny = x != 0.f ? (__float_as_uint(x) >> 16 & 0x8000u) | 1u : 0u;
+    uint32_t hi = __half_as_ushort(__float2half_rz(x));
+    const float rest = x - __half2float(__ushort_as_half((unsigned short)hi));
+    uint32_t lo = __half_as_ushort(__float2half_rn(rest));
+    if (!(fabsf(x) < INFINITY)) return hi;
+    if ((hi & 0x7fffu) == 0) hi = tiny;
+    if ((lo & 0x7fffu) == 0) lo = tiny;
+    return hi | lo << 16;
 }
 
-// v[i] summed over the 16 lanes of each half-warp, for i = 0..15: the lane with sl == i gets sum i.
-__device__ __forceinline__ float transpose_sum16(const float (&v)[16], int sl) {
-    float w8[8], w4[4], w2[2];
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) w8[i] = (sl & 8 ? v[i + 8] : v[i]) + __shfl_xor_sync(0xffffffffu, sl & 8 ? v[i] : v[i + 8], 8);
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) w4[i] = (sl & 4 ? w8[i + 4] : w8[i]) + __shfl_xor_sync(0xffffffffu, sl & 4 ? w8[i] : w8[i + 4], 4);
-    #pragma unroll
-    for (int i = 0; i < 2; ++i) w2[i] = (sl & 2 ? w4[i + 2] : w4[i]) + __shfl_xor_sync(0xffffffffu, sl & 2 ? w4[i] : w4[i + 2], 2);
-    return (sl & 1 ? w2[1] : w2[0]) + __shfl_xor_sync(0xffffffffu, sl & 1 ? w2[0] : w2[1], 1);
-}
-
-__global__ void __launch_bounds__(THREADS, 2) attn_paged_split_kernel(const PagedAttnArgs a) {
-    extern __shared__ __align__(128) uint8_t ring[];         // [WARPS][STAGES][K rows | V rows]
+template <bool WEIGHTS>
+__global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap map) {
+    extern __shared__ __align__(1024) uint8_t ring[];        // [WARPS][STAGES][K rows | V rows]
     __shared__ __align__(8) uint64_t full[WARPS][STAGES];
-    __shared__ int start[MAX_PAGED_BATCH + 1];
+    __shared__ int start[MAX_PAGED_BATCH + 1], length[MAX_PAGED_BATCH];
     __shared__ int warp_sum[WARPS];
-    __shared__ float s_stat[2][WARPS][4];                    // by segment parity: max and sum of both heads
-    __shared__ __align__(16) float s_acc[2][WARPS][GROUP][D];
+    __shared__ __align__(16) uint32_t s_q[WARPS][Q_WORDS];
+    __shared__ Part parts[WARPS][2];                         // [0]: of the warp's first unit, [1]: of its last
+    __shared__ __align__(16) float s_part[WARPS][2][GROUP * D];
     __shared__ int abort_flag, never_abort;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int hw = lane >> 4, sl = lane & 15;                // half-warp: rows of one parity; 8 channels a lane
-    const int hq = GROUP * a.kv.hkv;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
+    const int g8 = lane >> 2, j4 = lane & 3, head = j4 & 1;  // tile row or column, and the column pair's head
+    const int hkv = a.kv.hkv;
     if (tid == 0) {
         abort_flag = 0; never_abort = 0;
         for (int i = 0; i < WARPS * STAGES; ++i) mbar_init(&full[0][0] + i, 1);
         fence_mbar_init();
+        prefetch_tmap(&map);
     }
-    const PagedSplit sp = scan_lengths(a, start, warp_sum);   // its barriers publish the ring's too
+    if (tid < WARPS * 2) parts[tid >> 1][tid & 1].unit = -1;
+    const PagedSplit sp = scan_lengths(a, start, length, warp_sum);   // its barriers publish the above too
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (blockIdx.x == 0)
-        for (int b = tid; b < a.n; b += THREADS)
-            if (a.lengths[b] != row_length(a, b)) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
-    // rows without keys: zeros
-    for (int i = blockIdx.x; i < a.n_layers * a.n; i += gridDim.x) {
-        const int b = i % a.n;
-        if (start[b + 1] == start[b])
-            for (int j = tid; j < hq * D; j += THREADS) a.out[(size_t)i * hq * D + j] = 0.f;
+    if (sp.total == 0 || c >= sp.ctas) {
+        if (tid < 2) shared_of(a)[c * 2 + tid].nrec = 0;
+        return;
     }
-    const int c = blockIdx.x;
-    if (sp.total == 0 || c >= sp.ctas) return;
-    const long long g_begin = sp.begin(c), g_end = sp.begin(c + 1);
+    const long long c_begin = sp.begin(c), c_end = sp.begin(c + 1);
+    const int c_blocks = (int)(c_end - c_begin);             // at most 2^28 (64 layers, 8 heads, 2^30 rows over 148 ranges)
+    // this warp's blocks [g_begin, g_end) of the range
+    const long long g_begin = c_begin + c_blocks * warp / WARPS, g_end = c_begin + c_blocks * (warp + 1) / WARPS;
     const float qscale = 1.4426950408889634f * 0.08838834764831845f;   // log2(e)/sqrt(128)
     const int mask = (1 << a.kv.shift) - 1;
     uint8_t* const my_ring = ring + warp * (STAGES * STAGE);
     uint64_t* const my_full = full[warp];
+    uint32_t issued = 0, consumed = 0;
 
-    // ---- producer side of the warp: blocks g_begin + warp, + WARPS, ... of the range ----
-    PagedUnit u = paged_unit_of(start, a.n, a.kv.hkv, g_begin);
-    PagedUnit pu = u;
-    long long pg = g_begin + warp;                           // next block to copy
-    uint32_t issued = 0, consumed = 0, valid = 0;            // valid: bit per stage, the block was copied
-    int next_page = -1;
-    auto find_page = [&]() {                                 // page id of block pg (loaded ahead of its use)
-        if (pg >= g_end) return;
-        while (pg >= pu.off + pu.nblk) paged_next_unit(start, a.n, a.kv.hkv, pu);
-        next_page = __ldg(a.table + (size_t)pu.b * a.cols + ((int)(pg - pu.off) * BLK >> a.kv.shift));
-    };
-    auto produce = [&]() {
-        if (pg >= g_end) return;
-        const int stage = issued % STAGES;
-        const int t0 = (int)(pg - pu.off) * BLK;
-        const uint32_t bytes = min(BLK, row_length(a, pu.b) - t0) * (D * 2);
-        const bool ok = a.kv.has(next_page);
-        valid = ok ? valid | 1u << stage : valid & ~(1u << stage);
-        if (lane == 0) {
-            if (ok) {
-                const int layer = a.layer0 + pu.l;
-                mbar_arrive_expect_tx(&my_full[stage], 2 * bytes);
-                bulk_copy(my_ring + stage * STAGE, a.kv.row(next_page, layer, 0, pu.kh, t0 & mask), bytes, &my_full[stage]);
-                bulk_copy(my_ring + stage * STAGE + HALF_STAGE, a.kv.row(next_page, layer, 1, pu.kh, t0 & mask), bytes,
-                          &my_full[stage]);
-            } else {
-                mbar_arrive(&my_full[stage]);
-                atomicCAS(a.error, 0, PAGED_BAD_PAGE);
+    if (g_begin < g_end) {
+        // ---- producer side ----
+        PagedUnit u = paged_unit_of(start, a.n, hkv, g_begin);
+        PagedUnit pu = u;
+        long long pg = g_begin;                              // next block to copy
+        uint32_t valid = 0;                                  // bit per stage: the block was copied
+        int next_page = -1;
+        auto find_page = [&]() {                             // page id of block pg (loaded ahead of its use)
+            if (pg >= g_end) return;
+            if (pg >= pu.off + pu.nblk) paged_next_unit(start, a.n, hkv, pu);
+            next_page = __ldg(a.table + (size_t)pu.b * a.cols + ((int)(pg - pu.off) * BLK >> a.kv.shift));
+        };
+        auto produce = [&]() {
+            if (pg >= g_end) return;
+            const int stage = issued % STAGES;
+            const int t0 = (int)(pg - pu.off) * BLK;
+            const bool ok = a.kv.has(next_page);
+            valid = ok ? valid | 1u << stage : valid & ~(1u << stage);
+            if (lane == 0) {
+                if (ok) mbar_arrive_expect_tx(&my_full[stage], STAGE);
+                else { mbar_arrive(&my_full[stage]); atomicCAS(a.error, 0, PAGED_BAD_PAGE); }
             }
-        }
-        ++issued;
-        pg += WARPS;
+            __syncwarp();
+            if (ok && lane < 4) {
+                // lane: K or V, channel half. The pool's rows are one matrix, of planes ((page, layer), K|V, head)
+                const int kv = lane >> 1, half = lane & 1;
+                const int plane = ((next_page * a.kv.layers + a.layer0 + pu.l) * 2 + kv) * hkv + pu.kh;
+                tma_load_2d(my_ring + stage * STAGE + kv * HALF_STAGE + half * (HALF_STAGE / 2), &map, half * 64,
+                            (plane << a.kv.shift) + (t0 & mask), &my_full[stage]);
+            }
+            ++issued;
+            ++pg;
+            find_page();
+        };
         find_page();
-    };
-    find_page();
-    for (int i = 0; i < STAGES; ++i) produce();
+        for (int i = 0; i < STAGES; ++i) produce();
 
-    auto load_q = [&](const PagedUnit& w, float4 (&x)[2 * GROUP]) {
-        const size_t row = ((size_t)w.l * a.n + w.b) * hq + (size_t)w.kh * GROUP;
-        #pragma unroll
-        for (int i = 0; i < 2 * GROUP; ++i)
-            x[i] = __ldg(reinterpret_cast<const float4*>(a.q + (row + (i >> 1)) * D + sl * 8) + (i & 1));
-    };
-    float4 q_raw[2 * GROUP];
-    load_q(u, q_raw);
-    long long my_g = g_begin + warp;                         // next block of this warp to consume
-    int parity = 0;
-    for (long long g = g_begin; g < g_end; parity ^= 1) {
-        const int cnt = (int)(min(u.off + u.nblk, g_end) - g);
-        const int len = row_length(a, u.b);
-        float2 q[GROUP][4], acc[GROUP][4];
-        #pragma unroll
-        for (int i = 0; i < GROUP; ++i) {
-            const float4 x = q_raw[2 * i], y = q_raw[2 * i + 1];
-            q[i][0] = make_float2(x.x * qscale, x.y * qscale); q[i][1] = make_float2(x.z * qscale, x.w * qscale);
-            q[i][2] = make_float2(y.x * qscale, y.y * qscale); q[i][3] = make_float2(y.z * qscale, y.w * qscale);
-            #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][e] = make_float2(0.f, 0.f);
-        }
-        PagedUnit nu = u;                                    // the next segment's queries, loaded meanwhile
-        if (g + cnt < g_end) {
-            paged_next_unit(start, a.n, a.kv.hkv, nu);
-            load_q(nu, q_raw);
-        }
-        float m = -INFINITY, l = 0.f;                        // of head sl & 1, this lane's share of the sum
-        for (; my_g < g + cnt; my_g += WARPS) {
-            const int stage = consumed % STAGES;
-            bool got = mbar_wait(&my_full[stage], (consumed / STAGES) & 1, &abort_flag);
-            if (!got) { abort_flag = 1; atomicCAS(a.error, 0, WAIT_CODE); }
-            got = __all_sync(0xffffffffu, got);
-            const uint8_t* buf = my_ring + stage * STAGE;
-            const int rows = min(BLK, len - (int)(my_g - u.off) * BLK);
-            if (got && (valid >> stage & 1)) {
-                // row 2i + hw of the block and head gq: partial sums over this lane's 8 channels, then
-                // over the 16 lanes; the lane with sl == 2i + gq keeps the logit
-                float v[16];
+        // queries: lane's 8 channels of head lane / 16, loaded a unit ahead
+        float4 q_raw[2];
+        auto load_q = [&](const PagedUnit& w) {
+            const float* row = a.q + ((((size_t)w.l * a.n + w.b) * hkv + w.kh) * GROUP) * D + lane * 8;
+            q_raw[0] = __ldg(reinterpret_cast<const float4*>(row));
+            q_raw[1] = __ldg(reinterpret_cast<const float4*>(row) + 1);
+        };
+        load_q(u);
+        // shared-memory rows this lane names to ldmatrix (16-byte chunk x of row r sits at chunk
+        // x ^ (r % 8) of its 128-byte line); K: rows in the low bit of the matrix index, V: chunks
+        const int mi = lane >> 3, k_row = (lane & 7) + (mi & 1) * 8, v_row = (lane & 7) + (mi >> 1) * 8;
+        const uint32_t ring_addr = smem_u32(my_ring);
+        for (long long g = g_begin; g < g_end;) {
+            const int cnt = (int)(min(u.off + u.nblk, g_end) - g), blk0 = (int)(g - u.off);
+            const int len = length[u.b];
+            uint32_t qf[16];                                 // column g8: head (g8 / 2) % 2, its high or low half by g8 % 2
+            float unscale;                                   // logit = unscale * dot product, of head `head`
+            {
+                float v[8] = {q_raw[0].x, q_raw[0].y, q_raw[0].z, q_raw[0].w, q_raw[1].x, q_raw[1].y, q_raw[1].z, q_raw[1].w};
+                float top = 0.f;
                 #pragma unroll
-                for (int i = 0; i < BLK / 2; ++i) {
-                    float kf[8];
-                    unpack8(*reinterpret_cast<const uint4*>(buf + (2 * i + hw) * (D * 2) + sl * 16), kf);
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+                #pragma unroll
+                for (int o = 1; o <= 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                // scale = 2^(13 - exponent of top), at most 2^100
+                const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -87), 127);
+                const float scale = __uint_as_float((uint32_t)(13 - e + 127) << 23);
+                unscale = __shfl_sync(0xffffffffu, qscale * __uint_as_float((uint32_t)(e - 13 + 127) << 23), head * 16);
+                uint32_t h[8];
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) h[i] = split_half(v[i] * scale);
+                uint4* to = reinterpret_cast<uint4*>(&s_q[warp][lane * 8]);
+                to[0] = make_uint4(h[0], h[1], h[2], h[3]);
+                to[1] = make_uint4(h[4], h[5], h[6], h[7]);
+                __syncwarp();
+                // channels 16 k + 2 j4 + {0, 1} and + {8, 9} of step k
+                const uint2* from = reinterpret_cast<const uint2*>(&s_q[warp][(g8 >> 1 & 1) * D + 2 * j4]);
+                #pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint2 x = from[4 * i];
+                    qf[i] = __byte_perm(x.x, x.y, g8 & 1 ? 0x7632 : 0x5410);
+                }
+                __syncwarp();
+            }
+            PagedUnit nu = u;                                // the next unit's queries, loaded meanwhile
+            if (g + cnt < g_end) {
+                paged_next_unit(start, a.n, hkv, nu);
+                load_q(nu);
+            }
+            float m = -INFINITY, l = 0.f;                    // of head `head`: maximum - 14, this lane's share of the sum
+            float acc[8][4];                                 // [16-channel tile]: channels g8, g8 + 8; high and low columns of `head`
+            #pragma unroll
+            for (int i = 0; i < 8; ++i)
+                #pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+            for (int j = 0; j < cnt; ++j) {
+                const int stage = consumed % STAGES;
+                bool got = mbar_wait(&my_full[stage], (consumed / STAGES) & 1, &abort_flag);
+                if (!got) { abort_flag = 1; atomicCAS(a.error, 0, WAIT_CODE); }
+                got = __all_sync(0xffffffffu, got);
+                const int rows = min(BLK, len - (blk0 + j) * BLK);
+                if (got && (valid >> stage & 1)) {
+                    const uint32_t k_addr = ring_addr + stage * STAGE + k_row * 128, v_addr = ring_addr + stage * STAGE + HALF_STAGE + v_row * 128;
+                    // logits: rows g8 and g8 + 8 of the block, columns 2 j4 (high) and 2 j4 + 1 (low)
+                    float sc[2][4] = {};
                     #pragma unroll
-                    for (int gq = 0; gq < GROUP; ++gq) {
-                        float2 d = make_float2(0.f, 0.f);
+                    for (int k = 0; k < 8; ++k) {
+                        uint32_t kf[4];
+                        const int chunk = (2 * k + (mi >> 1)) & 7;
+                        ldmatrix4(kf, k_addr + (k >> 2) * (HALF_STAGE / 2) + ((chunk ^ (k_row & 7)) << 4));
+                        mma16816(sc[k & 1], kf, qf[2 * k], qf[2 * k + 1]);
+                    }
+                    float s0 = ((sc[0][0] + sc[1][0]) + (sc[0][1] + sc[1][1])) * unscale;
+                    float s1 = ((sc[0][2] + sc[1][2]) + (sc[0][3] + sc[1][3])) * unscale;
+                    if (rows < BLK) {
+                        // rows past the length: no logit, and zero V rows, whatever their page holds
+                        if (g8 >= rows) s0 = -INFINITY;
+                        if (g8 + 8 >= rows) s1 = -INFINITY;
+                        for (int i = rows * 8 + lane; i < BLK * 8; i += 32) {
+                            uint4* v = reinterpret_cast<uint4*>(my_ring + stage * STAGE + HALF_STAGE) + i;
+                            v[0] = make_uint4(0, 0, 0, 0);
+                            v[BLK * 8] = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();            // before the stage's next copy
+                        __syncwarp();
+                    }
+                    if (WEIGHTS && j4 < GROUP) {
+                        float* to = a.logits + (g + j) * (BLK * 2) + g8 * 2 + j4;
+                        to[0] = s0;
+                        to[16] = s1;
+                    }
+                    float mb = fmaxf(s0, s1);
+                    #pragma unroll
+                    for (int o = 4; o <= 16; o <<= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+                    mb -= 14.f;
+                    if (__any_sync(0xffffffffu, mb > m)) {
+                        const float mn = fmaxf(m, mb), scale = exp2_from(m, mn);
+                        m = mn;
+                        l *= scale;
                         #pragma unroll
-                        for (int e = 0; e < 4; ++e) d = ffma2(q[gq][e], make_float2(kf[2 * e], kf[2 * e + 1]), d);
-                        v[2 * i + gq] = d.x + d.y;
+                        for (int i = 0; i < 8; ++i)
+                            #pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[i][e] *= scale;
                     }
-                }
-                const int t = 2 * (sl >> 1) + hw;            // this lane's row of the block
-                const bool there = t < rows;
-                float s = transpose_sum16(v, sl);
-                if (!there) s = -INFINITY;                   // (stale bytes of the ring)
-                if (a.add_weights) a.logits[my_g * (BLK * 2) + t * 2 + (sl & 1)] = s;
-                float mb = s;
-                #pragma unroll
-                for (int o = 2; o <= 16; o <<= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
-                if (__any_sync(0xffffffffu, mb > m)) {
-                    const float mn = fmaxf(m, mb);
-                    const float scale = exp2_from(m, mn);
-                    m = mn;
-                    l *= scale;
-                    const float other = __shfl_xor_sync(0xffffffffu, scale, 1);
-                    const float sc0 = sl & 1 ? other : scale, sc1 = sl & 1 ? scale : other;
+                    const float p0 = g8 < rows ? exp2_from(s0, m) : 0.f, p1 = g8 + 8 < rows ? exp2_from(s1, m) : 0.f;
+                    l += p0 + p1;
+                    // this lane's operand: rows 2 j4 + {0, 1, 8, 9} of column g8 (head (g8 / 2) % 2, half g8 % 2)
+                    const uint32_t h0 = split_half(p0), h1 = split_half(p1);
+                    const int from = 8 * j4 + (g8 >> 1 & 1);
+                    const uint32_t x0 = __shfl_sync(0xffffffffu, h0, from), x1 = __shfl_sync(0xffffffffu, h0, from + 4);
+                    const uint32_t x2 = __shfl_sync(0xffffffffu, h1, from), x3 = __shfl_sync(0xffffffffu, h1, from + 4);
+                    const uint32_t pick = g8 & 1 ? 0x7632 : 0x5410;
+                    const uint32_t b0 = __byte_perm(x0, x1, pick), b1 = __byte_perm(x2, x3, pick);
                     #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        acc[0][e].x *= sc0; acc[0][e].y *= sc0;
-                        acc[1][e].x *= sc1; acc[1][e].y *= sc1;
+                    for (int i = 0; i < 8; ++i) {
+                        uint32_t vf[4];
+                        const int chunk = (2 * i + (mi & 1)) & 7;
+                        ldmatrix4_trans(vf, v_addr + (i >> 2) * (HALF_STAGE / 2) + ((chunk ^ (v_row & 7)) << 4));
+                        mma16816(acc[i], vf, b0, b1);
                     }
                 }
-                const float p = there ? exp2_from(s, m) : 0.f;
-                l += p;
-                #pragma unroll
-                for (int i = 0; i < BLK / 2; ++i) {
-                    uint4 vr = *reinterpret_cast<const uint4*>(buf + HALF_STAGE + (2 * i + hw) * (D * 2) + sl * 16);
-                    if (2 * i + hw >= rows) vr = make_uint4(0, 0, 0, 0);   // stale bytes count nothing, whatever they are
-                    float vf[8];
-                    unpack8(vr, vf);
-                    const float p0 = __shfl_sync(0xffffffffu, p, (lane & 16) + 2 * i);
-                    const float p1 = __shfl_sync(0xffffffffu, p, (lane & 16) + 2 * i + 1);
-                    #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 v2 = make_float2(vf[2 * e], vf[2 * e + 1]);
-                        acc[0][e] = ffma2(make_float2(p0, p0), v2, acc[0][e]);
-                        acc[1][e] = ffma2(make_float2(p1, p1), v2, acc[1][e]);
-                    }
+                __syncwarp();                                // the stage is read by all lanes
+                if (got) {
+                    ++consumed;
+                    produce();
                 }
             }
-            __syncwarp();                                    // the stage is read by all lanes
-            if (got) {
-                ++consumed;
-                produce();
+            // ---- the unit's part is done: column `head`; lanes j4 < 2 write channels g8, the others g8 + 8 ----
+            #pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            const int unit = (u.l * a.n + u.b) * hkv + u.kh;
+            const bool whole = cnt == u.nblk;
+            float* to = a.out + (size_t)unit * GROUP * D;
+            if (!whole) {
+                const int slot = g == g_begin ? 0 : 1;       // (a middle unit is whole)
+                to = s_part[warp][slot];
+                if (lane == 0) {
+                    Part& p = parts[warp][slot];
+                    p.unit = unit; p.blk0 = blk0; p.cnt = cnt; p.nblk = u.nblk;
+                }
+                if (lane < GROUP) { parts[warp][slot].m[lane] = m; parts[warp][slot].l[lane] = l; }
             }
-        }
-        // ---- merge the warps ----
-        #pragma unroll
-        for (int o = 2; o <= 16; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        #pragma unroll
-        for (int i = 0; i < GROUP; ++i)
             #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                acc[i][e].x += __shfl_xor_sync(0xffffffffu, acc[i][e].x, 16);
-                acc[i][e].y += __shfl_xor_sync(0xffffffffu, acc[i][e].y, 16);
-                if (hw == 0) *reinterpret_cast<float2*>(&s_acc[parity][warp][i][sl * 8 + 2 * e]) = acc[i][e];
+            for (int i = 0; i < 8; ++i) {
+                const float x = (j4 < 2 ? acc[i][0] + acc[i][1] : acc[i][2] + acc[i][3]);
+                to[head * D + 16 * i + g8 + (j4 < 2 ? 0 : 8)] = whole ? x / l : x;
             }
-        if (lane < 2) { s_stat[parity][warp][lane] = m; s_stat[parity][warp][2 + lane] = l; }
-        __syncthreads();                                     // (the other parity's buffers were read before it)
-        float M[GROUP], L[GROUP], o[GROUP];
-        #pragma unroll
-        for (int i = 0; i < GROUP; ++i) {
-            M[i] = s_stat[parity][0][i];
-            #pragma unroll
-            for (int w = 1; w < WARPS; ++w) M[i] = fmaxf(M[i], s_stat[parity][w][i]);
-            L[i] = 0.f; o[i] = 0.f;
-            #pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const float f = exp2_from(s_stat[parity][w][i], M[i]);
-                L[i] += f * s_stat[parity][w][2 + i];
-                o[i] += f * s_acc[parity][w][i][tid];
+            if (WEIGHTS && whole) {
+                const float M[GROUP] = {__shfl_sync(0xffffffffu, m, 0), __shfl_sync(0xffffffffu, m, 1)};
+                const float L[GROUP] = {__shfl_sync(0xffffffffu, l, 0), __shfl_sync(0xffffffffu, l, 1)};
+                __syncwarp();                                // the warp's own logits
+                add_weights(a, u.l, u.b, u.kh, len, 0, cnt, g, M, L, lane, 32);
             }
+            g += cnt;
+            u = nu;
         }
-        if (cnt == u.nblk) {
-            const size_t qrow = ((size_t)u.l * a.n + u.b) * hq + (size_t)u.kh * GROUP;
-            #pragma unroll
-            for (int i = 0; i < GROUP; ++i) a.out[(qrow + i) * D + tid] = o[i] / L[i];
-            if (a.add_weights) add_weights(a, u, g, cnt, M, L);
-        } else {
-            float* rec = a.records + ((size_t)c * 2 + (g != g_begin)) * PARTIAL_FLOATS;
-            if (tid < GROUP) { rec[tid] = M[tid]; rec[GROUP + tid] = L[tid]; }
-            #pragma unroll
-            for (int i = 0; i < GROUP; ++i) rec[4 + i * D + tid] = o[i];
-        }
-        g += cnt;
-        u = nu;
+        // drain: copies issued but not consumed (after an expired wait) must land before the CTA exits
+        for (; consumed < issued; ++consumed) mbar_wait(&my_full[consumed % STAGES], (consumed / STAGES) & 1, &never_abort, 500000000ull);
     }
-    // drain: copies issued but not consumed (after an expired wait) must land before the CTA exits
-    for (; consumed < issued; ++consumed) mbar_wait(&my_full[consumed % STAGES], (consumed / STAGES) & 1, &never_abort, 500000000ull);
+    __syncthreads();
+
+    // ---- merge the warps' parts, in order; consecutive parts of one unit are a group ----
+    bool have[2] = {false, false};                           // records of this range
+    for (int i = 0; i < WARPS * 2;) {
+        const int unit = parts[i >> 1][i & 1].unit;
+        if (unit < 0) { ++i; continue; }
+        const int begin = i, blk0 = parts[i >> 1][i & 1].blk0, nblk = parts[i >> 1][i & 1].nblk;
+        int cnt = 0, end = i;
+        float M[GROUP] = {-INFINITY, -INFINITY}, L[GROUP] = {0.f, 0.f}, o = 0.f;
+        for (; i < WARPS * 2; ++i) {
+            const Part& p = parts[i >> 1][i & 1];
+            if (p.unit < 0) continue;
+            if (p.unit != unit) break;
+            cnt += p.cnt;
+            end = i + 1;
+            #pragma unroll
+            for (int k = 0; k < GROUP; ++k) M[k] = fmaxf(M[k], p.m[k]);
+        }
+        const int kh = tid / D;                              // thread: column tid of [GROUP][D]
+        for (int k = begin; k < end; ++k) {
+            const Part& p = parts[k >> 1][k & 1];
+            if (p.unit < 0) continue;
+            const float f0 = exp2_from(p.m[0], M[0]), f1 = exp2_from(p.m[1], M[1]);
+            L[0] += f0 * p.l[0]; L[1] += f1 * p.l[1];
+            o += (kh ? f1 : f0) * s_part[k >> 1][k & 1][tid];
+        }
+        const int lb = unit / hkv, row_l = lb / a.n, row_b = lb - row_l * a.n, row_kh = unit - lb * hkv;
+        const long long off = paged_unit_offset(start, a.n, hkv, row_l, row_b, row_kh), g = off + blk0;
+        if (cnt == nblk) {
+            a.out[(size_t)unit * GROUP * D + tid] = o / L[kh];
+            if (WEIGHTS) add_weights(a, row_l, row_b, row_kh, length[row_b], blk0, cnt, g, M, L, tid, THREADS);
+        } else {
+            const int slot = g != c_begin;
+            float* rec = a.records + ((size_t)c * 2 + slot) * PARTIAL_FLOATS;
+            if (tid < GROUP) { rec[tid] = M[tid]; rec[GROUP + tid] = L[tid]; }
+            rec[4 + tid] = o;
+            if (tid == 0) {
+                Shared s;
+                s.first = sp.range_of(off);
+                s.nrec = sp.range_of(off + nblk - 1) - s.first + 1;
+                s.first_slot = off != sp.begin(s.first);
+                s.unit = unit; s.blk0 = blk0; s.cnt = cnt; s.g = g;
+                shared_of(a)[c * 2 + slot] = s;
+            }
+            have[slot] = true;
+        }
+    }
+    if (tid < 2 && !have[tid]) shared_of(a)[c * 2 + tid].nrec = 0;
 }
 
-// CTA c joins the unit whose first range is c, and adds the weights of the parts of shared units
-// that lie in range c.
-__global__ void __launch_bounds__(THREADS) attn_paged_join_kernel(const PagedAttnArgs a) {
-    __shared__ int start[MAX_PAGED_BATCH + 1];
-    __shared__ int warp_sum[WARPS];
+// CTA c joins the unit whose first range is c and, with weights, adds those of the parts of shared
+// units that lie in range c. Beside that, before the first launch is done: rows of length 0.
+__global__ void __launch_bounds__(JOIN_THREADS) attn_paged_join_kernel(const PagedAttnArgs a) {
     __shared__ float s_f[CTAS][GROUP];                       // factor of each record
-    __shared__ float red[2 * GROUP][WARPS];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x, hq = GROUP * a.kv.hkv;
-    const PagedSplit sp = scan_lengths(a, start, warp_sum);
+    __shared__ float red[2 * GROUP][JOIN_THREADS / 32];
+    __shared__ __align__(16) float s_sum[JOIN_GROUPS][GROUP * D];
+    static_assert(CTAS <= JOIN_THREADS && GROUP * D == JOIN_THREADS, "one record, and one column, a thread");
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
+    const int row_floats = GROUP * a.kv.hkv * D;
+    for (int b = tid; b < a.n && c == 0; b += JOIN_THREADS)
+        if (a.lengths[b] != row_length(a, b)) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
+    for (int i = c; i < a.n_layers * a.n; i += CTAS)
+        if (row_length(a, i % a.n) == 0)
+            for (int j = tid * 4; j < row_floats; j += JOIN_THREADS * 4)
+                *reinterpret_cast<float4*>(a.out + (size_t)i * row_floats + j) = make_float4(0.f, 0.f, 0.f, 0.f);
     asm volatile("griddepcontrol.wait;" ::: "memory");       // the split launch is complete and its stores visible
-    if (sp.total == 0 || c >= sp.ctas) return;
-    const long long g_begin = sp.begin(c), g_end = sp.begin(c + 1);
-    long long done = -1;
     for (int side = 0; side < 2; ++side) {
-        const PagedUnit u = paged_unit_of(start, a.n, a.kv.hkv, side ? g_end - 1 : g_begin);
-        if (u.off == done) continue;
-        done = u.off;
-        const int c_first = sp.range_of(u.off), c_last = sp.range_of(u.off + u.nblk - 1), nrec = c_last - c_first + 1;
-        if (nrec == 1 || (c != c_first && !a.add_weights)) continue;
-        // record i of the unit: range c_first + i; slot 0 but in the first range, unless it begins the range
-        const float* first = a.records + ((size_t)c_first * 2 + (u.off != sp.begin(c_first))) * PARTIAL_FLOATS;
-        const float* others = a.records + (size_t)c_first * 2 * PARTIAL_FLOATS;
+        const Shared s = shared_of(a)[c * 2 + side];
+        if (s.nrec == 0 || (s.first != c && !a.add_weights)) continue;
+        // record i of the unit: range first + i, slot 0 but in the first range
+        const float* first = a.records + ((size_t)s.first * 2 + s.first_slot) * PARTIAL_FLOATS;
+        const float* others = a.records + (size_t)s.first * 2 * PARTIAL_FLOATS;
         float M[GROUP] = {-INFINITY, -INFINITY}, L[GROUP] = {0.f, 0.f};
-        __syncthreads();                                     // s_f and red are free
-        for (int i = tid; i < nrec; i += THREADS) {
-            const float4 st = *reinterpret_cast<const float4*>(i ? others + (size_t)i * 2 * PARTIAL_FLOATS : first);
-            M[0] = fmaxf(M[0], st.x); M[1] = fmaxf(M[1], st.y);
-        }
+        float4 st = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+        if (tid < s.nrec) st = *reinterpret_cast<const float4*>(tid ? others + (size_t)tid * 2 * PARTIAL_FLOATS : first);
+        M[0] = st.x; M[1] = st.y;
         #pragma unroll
         for (int k = 0; k < GROUP; ++k) {
             #pragma unroll
             for (int x = 16; x >= 1; x >>= 1) M[k] = fmaxf(M[k], __shfl_xor_sync(0xffffffffu, M[k], x));
-            if (lane == 0) red[k][warp] = M[k];
         }
+        __syncthreads();                                     // s_f, red and s_sum are free
+        if (lane < GROUP) red[lane][warp] = lane ? M[1] : M[0];
         __syncthreads();
         #pragma unroll
         for (int k = 0; k < GROUP; ++k)
             #pragma unroll
-            for (int w = 0; w < WARPS; ++w) M[k] = fmaxf(M[k], red[k][w]);
-        for (int i = tid; i < nrec; i += THREADS) {
-            const float4 st = *reinterpret_cast<const float4*>(i ? others + (size_t)i * 2 * PARTIAL_FLOATS : first);
+            for (int w = 0; w < JOIN_THREADS / 32; ++w) M[k] = fmaxf(M[k], red[k][w]);
+        if (tid < s.nrec) {
             const float f0 = exp2_from(st.x, M[0]), f1 = exp2_from(st.y, M[1]);
-            s_f[i][0] = f0; s_f[i][1] = f1;
-            L[0] += f0 * st.z; L[1] += f1 * st.w;
+            s_f[tid][0] = f0; s_f[tid][1] = f1;
+            L[0] = f0 * st.z; L[1] = f1 * st.w;
         }
         #pragma unroll
         for (int k = 0; k < GROUP; ++k) {
             #pragma unroll
             for (int x = 16; x >= 1; x >>= 1) L[k] += __shfl_xor_sync(0xffffffffu, L[k], x);
-            if (lane == 0) red[GROUP + k][warp] = L[k];
         }
+        if (lane < GROUP) red[GROUP + lane][warp] = lane ? L[1] : L[0];
         __syncthreads();
         #pragma unroll
         for (int k = 0; k < GROUP; ++k) {
             L[k] = 0.f;
             #pragma unroll
-            for (int w = 0; w < WARPS; ++w) L[k] += red[GROUP + k][w];
+            for (int w = 0; w < JOIN_THREADS / 32; ++w) L[k] += red[GROUP + k][w];
         }
-        if (c == c_first) {
-            float o[GROUP];
-            #pragma unroll
-            for (int k = 0; k < GROUP; ++k) o[k] = s_f[0][k] * first[4 + k * D + tid];
+        if (s.first == c) {
+            // four columns a thread, every fourth record a group, then the groups in order
+            const int grp = tid / (GROUP * D / 4), col = tid % (GROUP * D / 4) * 4;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
             #pragma unroll 8
-            for (int i = 1; i < nrec; ++i) {
-                const float* rec = others + (size_t)i * 2 * PARTIAL_FLOATS + 4 + tid;
-                #pragma unroll
-                for (int k = 0; k < GROUP; ++k) o[k] += s_f[i][k] * rec[k * D];
+            for (int i = grp; i < s.nrec; i += JOIN_GROUPS) {
+                const float4 x = *reinterpret_cast<const float4*>((i ? others + (size_t)i * 2 * PARTIAL_FLOATS : first) + 4 + col);
+                const float f = s_f[i][col / D];
+                o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
             }
-            const size_t qrow = ((size_t)u.l * a.n + u.b) * hq + (size_t)u.kh * GROUP;
+            *reinterpret_cast<float4*>(&s_sum[grp][col]) = o;
+            __syncthreads();
+            float sum = 0.f;
             #pragma unroll
-            for (int k = 0; k < GROUP; ++k) a.out[(qrow + k) * D + tid] = o[k] / L[k];
+            for (int k = 0; k < JOIN_GROUPS; ++k) sum += s_sum[k][tid];
+            a.out[(size_t)s.unit * GROUP * D + tid] = sum / L[tid / D];
         }
         if (a.add_weights) {
-            const long long g = max(u.off, g_begin);
-            add_weights(a, u, g, (int)(min(u.off + u.nblk, g_end) - g), M, L);
+            const int lb = s.unit / a.kv.hkv, b = lb % a.n;
+            add_weights(a, lb / a.n, b, s.unit % a.kv.hkv, row_length(a, b), s.blk0, s.cnt, s.g, M, L, tid, JOIN_THREADS);
         }
     }
 }
 
 }  // namespace
 
-size_t paged_attn_record_bytes() { return (size_t)CTAS * 2 * PARTIAL_FLOATS * sizeof(float); }
+// Workspace: [records][shared][logits].
+static constexpr size_t RECORD_BYTES = (size_t)CTAS * 2 * PARTIAL_FLOATS * sizeof(float);
+static constexpr size_t SHARED_BYTES = (size_t)CTAS * 2 * sizeof(Shared);
+static_assert(RECORD_BYTES % 16 == 0 && SHARED_BYTES % 16 == 0, "each part 16-byte aligned");
 
 size_t paged_attn_workspace(int n, int n_layers, int hkv, int max_rows, bool weights) {
     const size_t blocks = (size_t)n * n_layers * hkv * ((max_rows + BLK - 1) / BLK);
-    return paged_attn_record_bytes() + (weights ? blocks * BLK * 2 * sizeof(float) : 0);
+    return RECORD_BYTES + SHARED_BYTES + (weights ? blocks * BLK * 2 * sizeof(float) : 0);
 }
 
-cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(attn_paged_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING);
+template <bool WEIGHTS>
+static cudaError_t launch_split(const PagedAttnArgs& a, const CUtensorMap& map, cudaStream_t s) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_paged_split_kernel<WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING);
     if (e != cudaSuccess) return e;
-    attn_paged_split_kernel<<<CTAS, THREADS, RING, s>>>(a);
+    attn_paged_split_kernel<WEIGHTS><<<CTAS, THREADS, RING, s>>>(a, map);
+    return cudaPeekAtLastError();
+}
+
+cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* workspace, cudaStream_t s) {
+    char* ws = static_cast<char*>(workspace);
+    a.records = reinterpret_cast<float*>(ws);
+    a.shared = ws + RECORD_BYTES;
+    a.logits = reinterpret_cast<float*>(ws + RECORD_BYTES + SHARED_BYTES);
+    const cudaError_t e = a.add_weights ? launch_split<true>(a, map, s) : launch_split<false>(a, map, s);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(CTAS); cfg.blockDim = dim3(THREADS); cfg.stream = s;
+    cfg.gridDim = dim3(CTAS); cfg.blockDim = dim3(JOIN_THREADS); cfg.stream = s;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;

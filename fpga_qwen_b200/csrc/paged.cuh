@@ -42,26 +42,40 @@ constexpr int PAGED_BLK = 16;                 // cache rows per block (the small
 
 struct PagedUnit { int l, b, kh, nblk; long long off; };   // blocks [off, off + nblk) of the call
 
+// a / b of non-negative values; a 64-bit division costs the kernels' prologues some hundred cycles.
+QA_HD long long paged_div(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 struct PagedSplit {
-    long long total;                          // blocks of the call
-    int ctas;                                 // ranges in use
-    QA_HD long long begin(int c) const { return (long long)c * total / ctas; }
-    // range that holds block g: the largest c with begin(c) <= g
-    QA_HD int range_of(long long g) const { return (int)(((g + 1) * ctas - 1) / total); }
+    long long total, per;                     // blocks of the call; of a range, the first `rem` of which hold one more
+    int ctas, rem;                            // ranges in use
+    QA_HD long long begin(int c) const { return c * per + (c < rem ? c : rem); }
+    QA_HD int range_of(long long g) const {   // range that holds block g
+        const long long edge = rem * (per + 1);
+        return (int)(g < edge ? paged_div(g, per + 1) : rem + paged_div(g - edge, per));
+    }
 };
 
 QA_HD PagedSplit paged_split(long long total, int max_ctas, int min_blocks) {
     PagedSplit s;
     s.total = total;
-    const long long fit = total / min_blocks;
+    const long long fit = paged_div(total, min_blocks);
     s.ctas = fit < 1 ? 1 : fit < max_ctas ? (int)fit : max_ctas;
+    s.per = paged_div(total, s.ctas);
+    s.rem = (int)(total - s.per * s.ctas);
     return s;
+}
+
+// First block of unit (l, b, kh).
+QA_HD long long paged_unit_offset(const int* start, int n, int hkv, int l, int b, int kh) {
+    return (long long)hkv * start[n] * l + (long long)hkv * start[b] + (long long)kh * (start[b + 1] - start[b]);
 }
 
 QA_HD PagedUnit paged_unit_of(const int* start, int n, int hkv, long long g) {
     const long long layer_blocks = (long long)hkv * start[n];
     PagedUnit u;
-    u.l = (int)(g / layer_blocks);
+    u.l = (int)paged_div(g, layer_blocks);
     const long long r = g - u.l * layer_blocks;
     int lo = 0, hi = n;                       // largest b with hkv * start[b] <= r (rows of length 0 have no width)
     while (hi - lo > 1) {
@@ -71,7 +85,7 @@ QA_HD PagedUnit paged_unit_of(const int* start, int n, int hkv, long long g) {
     u.b = lo;
     u.nblk = start[lo + 1] - start[lo];
     const long long rr = r - (long long)hkv * start[lo];
-    u.kh = (int)(rr / u.nblk);
+    u.kh = (int)paged_div(rr, u.nblk);
     u.off = g - (rr - (long long)u.kh * u.nblk);
     return u;
 }

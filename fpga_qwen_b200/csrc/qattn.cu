@@ -32,6 +32,10 @@ int nccl_send_recv_bytes(void* comm, void* buf, size_t bytes, int peer, bool sen
 int nccl_all_gather_bytes(void* comm, const void* send, void* recv, size_t bytes, cudaStream_t s, std::string& err);
 }  // namespace qattn
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
 struct qa_ctx {
     qa_config cfg{};
     int hq = 0, hkv = 0;                   // local heads
@@ -56,6 +60,7 @@ struct qa_ctx {
     float* staging = nullptr;
     size_t staging_floats = 0, io_out_floats = 0, io_in_floats = 0;
     char* io_pin = nullptr;                // io_host: pinned [error block][outputs][inputs] of packed copies
+    EncodeTiledFn encode = nullptr;        // cuTensorMapEncodeTiled
     CUtensorMap kv_map{};                  // 3-D view {128 ch, ctx, planes} of the KV store, 64x128 boxes
     int* error = nullptr;                  // device error block (qattn_common.cuh: ERR_*), at io_dev
     int* prefill_tiles = nullptr;          // work-item counter of the persistent prefill kernel
@@ -334,22 +339,17 @@ int io_host_call(qa_ctx* ctx, int seq, int layer, int n_layers, const IoCall& c,
     return QA_OK;
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 // TMA descriptor of the KV store: planes of [ctx][128] FP16 rows; rows past ctx read as zero.
 int make_kv_map(qa_ctx* ctx) {
-    EncodeTiledFn encode = nullptr;
     cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", reinterpret_cast<void**>(&encode), cudaEnableDefault, &q) !=
-            cudaSuccess || !encode)
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", reinterpret_cast<void**>(&ctx->encode), cudaEnableDefault, &q) !=
+            cudaSuccess || !ctx->encode)
         return fail(ctx, QA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
     const cuuint64_t planes = (cuuint64_t)ctx->cfg.max_seqs * ctx->cfg.n_layers * 2 * ctx->hkv;
     cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)ctx->cfg.context, planes};
     cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)ctx->cfg.context * D * 2};
     cuuint32_t box[3] = {64, 128, 1}, elem[3] = {1, 1, 1};
-    CUresult r = encode(&ctx->kv_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, ctx->kv.base, dims, strides, box, elem,
+    CUresult r = ctx->encode(&ctx->kv_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, ctx->kv.base, dims, strides, box, elem,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(ctx, QA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
@@ -1525,6 +1525,19 @@ int check_pages(qa_ctx* ctx, const qa_pages* p, const int* table, int cols, bool
     return QA_OK;
 }
 
+// TMA descriptor of a pool: its rows as one matrix [rows][128], in boxes of 16 rows x 64 channels.
+int make_pages_map(qa_ctx* ctx, const PagedKV& kv, CUtensorMap* map) {
+    const cuuint64_t rows = ((cuuint64_t)kv.n_pages * kv.layers * 2 * kv.hkv) << kv.shift;
+    if (rows > (cuuint64_t)INT32_MAX) return fail(ctx, QA_ERR_UNSUPPORTED, "a pool of %llu rows (at most 2^31 - 1)", (unsigned long long)rows);
+    cuuint64_t dims[2] = {(cuuint64_t)D, rows}, strides[1] = {(cuuint64_t)D * 2};
+    cuuint32_t box[2] = {64, PAGED_BLK}, elem[2] = {1, 1};
+    const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, kv.base, dims, strides, box, elem,
+                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ctx, QA_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return QA_OK;
+}
+
 int check_paged_batch(qa_ctx* ctx, int n) {
     if (n < 1 || n > QA_MAX_PAGED_BATCH)
         return fail(ctx, QA_ERR_INVALID, "batch of %d sequences (1..%d)", n, QA_MAX_PAGED_BATCH);
@@ -1613,9 +1626,9 @@ int qa_paged_attn(qa_ctx* ctx, const qa_pages* pages, const int* table, int tabl
                     workspace_bytes, need);
     QA_CUDA(cudaSetDevice(ctx->cfg.device));
     a.table = table; a.cols = table_cols; a.lengths = lengths; a.n = n; a.add_weights = add_weights != 0;
-    a.records = static_cast<float*>(workspace);
-    a.logits = reinterpret_cast<float*>(static_cast<char*>(workspace) + paged_attn_record_bytes());
     a.error = ctx->error;
+    CUtensorMap map;
+    if ((st = make_pages_map(ctx, a.kv, &map))) return st;
     const size_t qn = (size_t)n * ctx->hq * D;
     IoCall c;
     c.in[0] = q; c.in_floats[0] = qn;
@@ -1623,7 +1636,7 @@ int qa_paged_attn(qa_ctx* ctx, const qa_pages* pages, const int* table, int tabl
     c.inputs_read_once = decode_inputs_read_once(n_layers, n, ctx->hkv);
     return run_call(ctx, -1, layer, n_layers, c, [&](int l0, int nl, const float* const* din, float* const* dout) {
         a.q = din[0]; a.out = dout[0]; a.layer0 = l0; a.n_layers = nl;
-        const cudaError_t e = launch_paged_attn(a, ctx->stream);
+        const cudaError_t e = launch_paged_attn(a, map, workspace, ctx->stream);
         if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, e, "paged_attn"); }
         return after_launch(ctx, -1, "paged_attn");
     });

@@ -230,14 +230,16 @@ struct PagedAttnArgs {
     PagedKV kv;
     const int* table; int cols; const int* lengths;
     int n, layer0, n_layers, add_weights;
-    float* records;                           // workspace: [ctas][2][PARTIAL_FLOATS]
-    float* logits;                            // workspace with add_weights: [16-row block][16][2]
+    // workspace, laid out by the launcher
+    float* records;                           // [ranges][2][PARTIAL_FLOATS]
+    void* shared;                             // [ranges][2] parts of units shared between ranges
+    float* logits;                            // with add_weights: [16-row block][16][2]
     int* error;
 };
 constexpr int MAX_PAGED_BATCH = 1024;
 size_t paged_attn_workspace(int n, int n_layers, int hkv, int max_rows, bool add_weights);
-size_t paged_attn_record_bytes();
-cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s);
+// map: the pool's rows as one matrix [rows][128], boxes of 16 rows x 64 channels, 128-byte swizzle.
+cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* workspace, cudaStream_t s);
 
 struct PagedEvictArgs {
     PagedKV kv;

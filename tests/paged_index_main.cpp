@@ -1,7 +1,7 @@
 // Walks the index arithmetic of the paged kernels (fpga_qwen_b200/csrc/paged.cuh) on the CPU, the way
-// the kernels do: every block of every unit is taken by exactly one range, at most two units of a
-// range are shared, every shared unit's records are found again by the join, and every place and
-// every workspace index lies inside its buffer. Prints "ok" or the first violation.
+// the kernels do: every block of every unit is taken by exactly one warp, at most two units of a
+// warp's part and of a range are shared, the parts and records of every shared unit are found
+// again in order, and every place and every workspace index lies inside its buffer. Prints "ok" or the first violation.
 #include <algorithm>
 #include <cstdio>
 #include <cstdlib>
@@ -19,7 +19,11 @@ using namespace qattn;
         if (!(cond)) { std::printf("line %d: %s\n", __LINE__, #cond); std::exit(1); } \
     } while (0)
 
-static void walk(const std::vector<int>& lengths, int cols, int shift, int layers, int hkv, int max_ctas, int min_blocks) {
+// One part of a unit that a warp does not finish alone, and the record of a range.
+struct Part { long long off = -1; long long g = 0; int cnt = 0, nblk = 0; };
+
+static void walk(const std::vector<int>& lengths, int cols, int shift, int layers, int hkv, int max_ctas, int min_blocks,
+                 int warps) {
     const int n = (int)lengths.size();
     std::vector<int> start(n + 1, 0);
     for (int b = 0; b < n; ++b) {
@@ -32,49 +36,72 @@ static void walk(const std::vector<int>& lengths, int cols, int shift, int layer
     const long long bound = (long long)n * layers * hkv * (((cols << shift) + PAGED_BLK - 1) / PAGED_BLK);
     CHECK(sp.total <= bound);                                   // logits [total * 16][2] fit the workspace
     if (!sp.total) return;
-    long long seen = 0;
-    std::map<std::pair<int, int>, long long> record;            // (range, slot) -> unit offset
+    long long seen = 0, whole_blocks = 0;
+    std::map<std::pair<int, int>, Part> record;                 // (range, slot)
     for (int c = 0; c < sp.ctas; ++c) {
-        const long long g0 = sp.begin(c), g1 = sp.begin(c + 1);
-        CHECK(g0 < g1 && g0 == seen);
-        CHECK(sp.range_of(g0) == c && sp.range_of(g1 - 1) == c);
-        PagedUnit u = paged_unit_of(start.data(), n, hkv, g0);
-        for (long long g = g0; g < g1;) {
-            if (g != g0) paged_next_unit(start.data(), n, hkv, u);
-            const PagedUnit w = paged_unit_of(start.data(), n, hkv, g);
-            CHECK(w.l == u.l && w.b == u.b && w.kh == u.kh && w.nblk == u.nblk && w.off == u.off);
-            CHECK(u.l >= 0 && u.l < layers && u.b >= 0 && u.b < n && u.kh >= 0 && u.kh < hkv && u.nblk > 0);
-            CHECK(u.off <= g && g < u.off + u.nblk);
-            const long long cnt = std::min(u.off + u.nblk, g1) - g;
-            const int t_last = ((int)(g - u.off + cnt) - 1) * PAGED_BLK;
-            CHECK(t_last < lengths[u.b] && (t_last >> shift) < cols);
-            if (cnt != u.nblk) {
-                const int slot = g != g0;
-                CHECK(record.emplace(std::make_pair(c, slot), u.off).second);
+        const long long c0 = sp.begin(c), c1 = sp.begin(c + 1);
+        CHECK(c0 < c1 && c0 == seen && c1 - c0 <= 1 << 28);
+        CHECK(sp.range_of(c0) == c && sp.range_of(c1 - 1) == c);
+        const int blocks = (int)(c1 - c0);
+        std::vector<Part> parts(warps * 2);
+        for (int w = 0; w < warps; ++w) {
+            const long long g0 = c0 + blocks * w / warps, g1 = c0 + blocks * (w + 1) / warps;
+            CHECK(g0 == seen);
+            if (g0 >= g1) continue;
+            PagedUnit u = paged_unit_of(start.data(), n, hkv, g0);
+            for (long long g = g0; g < g1;) {
+                if (g != g0) paged_next_unit(start.data(), n, hkv, u);
+                const PagedUnit x = paged_unit_of(start.data(), n, hkv, g);
+                CHECK(x.l == u.l && x.b == u.b && x.kh == u.kh && x.nblk == u.nblk && x.off == u.off);
+                CHECK(u.l >= 0 && u.l < layers && u.b >= 0 && u.b < n && u.kh >= 0 && u.kh < hkv && u.nblk > 0);
+                CHECK(u.off <= g && g < u.off + u.nblk);
+                CHECK(paged_unit_offset(start.data(), n, hkv, u.l, u.b, u.kh) == u.off);
+                const long long cnt = std::min(u.off + u.nblk, g1) - g;
+                const int t_last = ((int)(g - u.off + cnt) - 1) * PAGED_BLK;
+                CHECK(t_last < lengths[u.b] && (t_last >> shift) < cols);
+                if (cnt == u.nblk) {
+                    whole_blocks += cnt;
+                } else {
+                    Part& p = parts[w * 2 + (g != g0)];
+                    CHECK(p.off < 0);
+                    p.off = u.off; p.g = g; p.cnt = (int)cnt; p.nblk = u.nblk;
+                }
+                seen += cnt;
+                g += cnt;
             }
-            seen += cnt;
-            g += cnt;
+        }
+        for (int i = 0; i < warps * 2;) {                       // the merge of the warps' parts
+            if (parts[i].off < 0) { ++i; continue; }
+            Part sum = parts[i];
+            sum.cnt = 0;
+            for (; i < warps * 2; ++i) {
+                if (parts[i].off < 0) continue;
+                if (parts[i].off != sum.off) break;
+                CHECK(parts[i].g == sum.g + sum.cnt);
+                sum.cnt += parts[i].cnt;
+            }
+            if (sum.cnt == sum.nblk) whole_blocks += sum.cnt;
+            else CHECK(record.emplace(std::make_pair(c, sum.g != c0 ? 1 : 0), sum).second);
         }
     }
     CHECK(seen == sp.total);
-    size_t found = 0;
-    for (int c = 0; c < sp.ctas; ++c) {                         // the join
-        long long done = -1;
-        for (int side = 0; side < 2; ++side) {
-            const PagedUnit u = paged_unit_of(start.data(), n, hkv, side ? sp.begin(c + 1) - 1 : sp.begin(c));
-            if (u.off == done) continue;
-            done = u.off;
-            const int first = sp.range_of(u.off), last = sp.range_of(u.off + u.nblk - 1);
-            CHECK(first <= c && c <= last);
-            if (first == last || c != first) continue;
-            for (int r = first; r <= last; ++r) {
-                const auto it = record.find({r, r == first && u.off != sp.begin(r) ? 1 : 0});
-                CHECK(it != record.end() && it->second == u.off);
-                ++found;
-            }
+    std::map<std::pair<int, int>, Part> left = record;
+    for (const auto& r : record) {                              // the join: by the unit's first range, in order
+        const Part& p = r.second;
+        const int first = sp.range_of(p.off), nrec = sp.range_of(p.off + p.nblk - 1) - first + 1;
+        CHECK(nrec >= 2 && first <= r.first.first && r.first.first < first + nrec);
+        if (first != r.first.first) continue;
+        long long at = p.off;
+        for (int i = 0; i < nrec; ++i) {
+            const auto it = left.find({first + i, i == 0 && p.off != sp.begin(first) ? 1 : 0});
+            CHECK(it != left.end() && it->second.off == p.off && it->second.g == at);
+            at += it->second.cnt;
+            left.erase(it);
         }
+        CHECK(at == p.off + p.nblk);
+        whole_blocks += p.nblk;
     }
-    CHECK(found == record.size());                              // every shared unit joined once
+    CHECK(left.empty() && whole_blocks == sp.total);            // every unit finished once
 }
 
 int main() {
@@ -93,8 +120,8 @@ int main() {
                             for (int& x : len) x = pick(0, 3) ? 0 : pick(-5, 2 * most);    // outside the table: as empty
                         std::vector<int> valid(len);
                         for (int& x : valid) x = paged_length(x, cols, shift);
-                        walk(valid, cols, shift, layers, hkv, 296, 4);
-                        walk(valid, cols, shift, layers, hkv, pick(1, 600), pick(1, 16));
+                        walk(valid, cols, shift, layers, hkv, 148, 8, 8);
+                        walk(valid, cols, shift, layers, hkv, pick(1, 600), pick(1, 16), pick(1, 16));
                     }
     // places: every combination of bad and good length, sequence, position and page id
     for (int shift = 4; shift <= 9; ++shift) {
