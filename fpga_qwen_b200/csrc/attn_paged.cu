@@ -67,6 +67,7 @@ constexpr int WAIT_CODE = 43;                 // error code of an expired wait
 struct Part {
     int unit;                                 // (l * n + b) * hkv + kh, or -1: none
     int blk0, cnt, nblk;                      // blocks [blk0, blk0 + cnt) of the unit's nblk
+    long long g;                              // its first block in the call
     float m[GROUP], l[GROUP];
 };
 // The joining launch's view of a range's part of a shared unit.
@@ -194,8 +195,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
         prefetch_tmap(&map);
     }
     if (tid < WARPS * 2) parts[tid >> 1][tid & 1].unit = -1;
-    const PagedSplit sp = scan_lengths(a, start, length, warp_sum);   // its barriers publish the above too
+    asm volatile("griddepcontrol.wait;" ::: "memory");       // what ran before is complete
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const PagedSplit sp = scan_lengths(a, start, length, warp_sum);   // its barriers publish the above too
     if (sp.total == 0 || c >= sp.ctas) {
         if (tid < 2) shared_of(a)[c * 2 + tid].nrec = 0;
         return;
@@ -211,40 +213,45 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
     uint32_t issued = 0, consumed = 0;
 
     if (g_begin < g_end) {
-        // ---- producer side ----
-        PagedUnit u = paged_unit_of(start, a.n, hkv, g_begin);
-        PagedUnit pu = u;
-        long long pg = g_begin;                              // next block to copy
-        uint32_t valid = 0;                                  // bit per stage: the block was copied
-        int next_page = -1;
-        auto find_page = [&]() {                             // page id of block pg (loaded ahead of its use)
-            if (pg >= g_end) return;
-            if (pg >= pu.off + pu.nblk) paged_next_unit(start, a.n, hkv, pu);
-            next_page = __ldg(a.table + (size_t)pu.b * a.cols + ((int)(pg - pu.off) * BLK >> a.kv.shift));
+        // ---- producer side: 32 blocks are looked up at a time, one a lane, a batch ahead ----
+        PagedUnit u = paged_unit_of(start, a.n, hkv, min(g_begin + lane, g_end - 1));
+        int page_next = -1, place_next = 0;                  // next batch: page id, first row within the page's K rows of the head
+        auto look_up = [&](const PagedUnit& w, long long g) {
+            const int t0 = (int)(g - w.off) * BLK;
+            page_next = __ldg(a.table + (size_t)w.b * a.cols + (t0 >> a.kv.shift));
+            place_next = (((a.layer0 + w.l) * 2 * hkv + w.kh) << a.kv.shift) + (t0 & mask);
         };
+        // row of the block's K in the pool's matrix of planes ((page, layer), K|V, head); -1: no such page
+        auto place = [&]() { return a.kv.has(page_next) ? ((page_next * a.kv.layers * 2 * hkv) << a.kv.shift) + place_next : -1; };
+        look_up(u, min(g_begin + lane, g_end - 1));
+        auto from_first = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+        u.l = from_first(u.l); u.b = from_first(u.b); u.kh = from_first(u.kh); u.nblk = from_first(u.nblk);
+        u.off = __shfl_sync(0xffffffffu, u.off, 0);          // the unit of g_begin
+        int rows_now = place();                              // of the batch being copied
+        const int n_blocks = (int)(g_end - g_begin);
+        uint32_t valid = 0;                                  // bit per stage: the block was copied
         auto produce = [&]() {
-            if (pg >= g_end) return;
-            const int stage = issued % STAGES;
-            const int t0 = (int)(pg - pu.off) * BLK;
-            const bool ok = a.kv.has(next_page);
+            if ((int)issued >= n_blocks) return;
+            if ((issued & 31) == 0) {
+                if (issued) rows_now = place();
+                const long long next = g_begin + issued + 32 + lane;
+                if (next - lane < g_end) look_up(paged_unit_of(start, a.n, hkv, min(next, g_end - 1)), min(next, g_end - 1));
+            }
+            const int stage = issued % STAGES, row = __shfl_sync(0xffffffffu, rows_now, issued & 31);
+            const bool ok = row >= 0;
             valid = ok ? valid | 1u << stage : valid & ~(1u << stage);
             if (lane == 0) {
                 if (ok) mbar_arrive_expect_tx(&my_full[stage], STAGE);
                 else { mbar_arrive(&my_full[stage]); atomicCAS(a.error, 0, PAGED_BAD_PAGE); }
             }
             __syncwarp();
-            if (ok && lane < 4) {
-                // lane: K or V, channel half. The pool's rows are one matrix, of planes ((page, layer), K|V, head)
+            if (ok && lane < 4) {                            // lane: K or V, channel half
                 const int kv = lane >> 1, half = lane & 1;
-                const int plane = ((next_page * a.kv.layers + a.layer0 + pu.l) * 2 + kv) * hkv + pu.kh;
                 tma_load_2d(my_ring + stage * STAGE + kv * HALF_STAGE + half * (HALF_STAGE / 2), &map, half * 64,
-                            (plane << a.kv.shift) + (t0 & mask), &my_full[stage]);
+                            row + (kv * hkv << a.kv.shift), &my_full[stage]);
             }
             ++issued;
-            ++pg;
-            find_page();
         };
-        find_page();
         for (int i = 0; i < STAGES; ++i) produce();
 
         // queries: lane's 8 channels of head lane / 16, loaded a unit ahead
@@ -385,7 +392,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
                 to = s_part[warp][slot];
                 if (lane == 0) {
                     Part& p = parts[warp][slot];
-                    p.unit = unit; p.blk0 = blk0; p.cnt = cnt; p.nblk = u.nblk;
+                    p.unit = unit; p.blk0 = blk0; p.cnt = cnt; p.nblk = u.nblk; p.g = g;
                 }
                 if (lane < GROUP) { parts[warp][slot].m[lane] = m; parts[warp][slot].l[lane] = l; }
             }
@@ -408,42 +415,55 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
     }
     __syncthreads();
 
-    // ---- merge the warps' parts, in order; consecutive parts of one unit are a group ----
+    // ---- merge the warps' parts: those of one unit are neighbours in the order of the blocks ----
+    // every warp holds all parts, one a lane; thread: column tid of [GROUP][D]
+    Part p;
+    p.unit = -1;
+    if (lane < WARPS * 2) p = parts[lane >> 1][lane & 1];
+    unsigned left = __ballot_sync(0xffffffffu, p.unit >= 0);
     bool have[2] = {false, false};                           // records of this range
-    for (int i = 0; i < WARPS * 2;) {
-        const int unit = parts[i >> 1][i & 1].unit;
-        if (unit < 0) { ++i; continue; }
-        const int begin = i, blk0 = parts[i >> 1][i & 1].blk0, nblk = parts[i >> 1][i & 1].nblk;
-        int cnt = 0, end = i;
-        float M[GROUP] = {-INFINITY, -INFINITY}, L[GROUP] = {0.f, 0.f}, o = 0.f;
-        for (; i < WARPS * 2; ++i) {
-            const Part& p = parts[i >> 1][i & 1];
-            if (p.unit < 0) continue;
-            if (p.unit != unit) break;
-            cnt += p.cnt;
-            end = i + 1;
+    while (left) {
+        const int first = __ffs(left) - 1;
+        const int unit = __shfl_sync(0xffffffffu, p.unit, first), blk0 = __shfl_sync(0xffffffffu, p.blk0, first);
+        const int nblk = __shfl_sync(0xffffffffu, p.nblk, first);
+        const long long g = __shfl_sync(0xffffffffu, p.g, first);
+        const bool mine = p.unit == unit;
+        const unsigned group = __ballot_sync(0xffffffffu, mine);
+        left &= ~group;
+        const int cnt = __reduce_add_sync(0xffffffffu, mine ? p.cnt : 0);
+        float M[GROUP], L[GROUP], f[GROUP];
+        #pragma unroll
+        for (int k = 0; k < GROUP; ++k) {
+            M[k] = mine ? p.m[k] : -INFINITY;
             #pragma unroll
-            for (int k = 0; k < GROUP; ++k) M[k] = fmaxf(M[k], p.m[k]);
+            for (int x = WARPS; x >= 1; x >>= 1) M[k] = fmaxf(M[k], __shfl_xor_sync(0xffffffffu, M[k], x, WARPS * 2));
+            M[k] = __shfl_sync(0xffffffffu, M[k], 0);
+            f[k] = mine ? exp2_from(p.m[k], M[k]) : 0.f;
+            L[k] = mine ? f[k] * p.l[k] : 0.f;
+            #pragma unroll
+            for (int x = WARPS; x >= 1; x >>= 1) L[k] += __shfl_xor_sync(0xffffffffu, L[k], x, WARPS * 2);
+            L[k] = __shfl_sync(0xffffffffu, L[k], 0);
         }
-        const int kh = tid / D;                              // thread: column tid of [GROUP][D]
-        for (int k = begin; k < end; ++k) {
-            const Part& p = parts[k >> 1][k & 1];
-            if (p.unit < 0) continue;
-            const float f0 = exp2_from(p.m[0], M[0]), f1 = exp2_from(p.m[1], M[1]);
-            L[0] += f0 * p.l[0]; L[1] += f1 * p.l[1];
-            o += (kh ? f1 : f0) * s_part[k >> 1][k & 1][tid];
+        const bool head1 = tid >= D;                         // (a warp's columns are of one head)
+        float o = 0.f;
+        #pragma unroll
+        for (int k = 0; k < WARPS * 2; ++k) {
+            const float fk = __shfl_sync(0xffffffffu, head1 ? f[1] : f[0], k);
+            if (group >> k & 1) o += fk * s_part[k >> 1][k & 1][tid];
         }
-        const int lb = unit / hkv, row_l = lb / a.n, row_b = lb - row_l * a.n, row_kh = unit - lb * hkv;
-        const long long off = paged_unit_offset(start, a.n, hkv, row_l, row_b, row_kh), g = off + blk0;
         if (cnt == nblk) {
-            a.out[(size_t)unit * GROUP * D + tid] = o / L[kh];
-            if (WEIGHTS) add_weights(a, row_l, row_b, row_kh, length[row_b], blk0, cnt, g, M, L, tid, THREADS);
+            a.out[(size_t)unit * GROUP * D + tid] = o / (head1 ? L[1] : L[0]);
+            if (WEIGHTS) {
+                const int lb = unit / hkv, row_l = lb / a.n, row_b = lb - row_l * a.n, row_kh = unit - lb * hkv;
+                add_weights(a, row_l, row_b, row_kh, length[row_b], 0, cnt, g, M, L, tid, THREADS);
+            }
         } else {
             const int slot = g != c_begin;
             float* rec = a.records + ((size_t)c * 2 + slot) * PARTIAL_FLOATS;
             if (tid < GROUP) { rec[tid] = M[tid]; rec[GROUP + tid] = L[tid]; }
             rec[4 + tid] = o;
             if (tid == 0) {
+                const long long off = g - blk0;
                 Shared s;
                 s.first = sp.range_of(off);
                 s.nrec = sp.range_of(off + nblk - 1) - s.first + 1;
@@ -549,12 +569,22 @@ size_t paged_attn_workspace(int n, int n_layers, int hkv, int max_rows, bool wei
     return RECORD_BYTES + SHARED_BYTES + (weights ? blocks * BLK * 2 * sizeof(float) : 0);
 }
 
+// A launch whose CTAs may start while the launch before it ends; they wait for its end themselves.
+template <class... Params, class... Args>
+static cudaError_t launch_dependent(void (*kernel)(Params...), int threads, size_t smem, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(CTAS); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <bool WEIGHTS>
 static cudaError_t launch_split(const PagedAttnArgs& a, const CUtensorMap& map, cudaStream_t s) {
     const cudaError_t e = cudaFuncSetAttribute(attn_paged_split_kernel<WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING);
-    if (e != cudaSuccess) return e;
-    attn_paged_split_kernel<WEIGHTS><<<CTAS, THREADS, RING, s>>>(a, map);
-    return cudaPeekAtLastError();
+    return e != cudaSuccess ? e : launch_dependent(attn_paged_split_kernel<WEIGHTS>, THREADS, RING, s, a, map);
 }
 
 cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* workspace, cudaStream_t s) {
@@ -563,14 +593,7 @@ cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* wor
     a.shared = ws + RECORD_BYTES;
     a.logits = reinterpret_cast<float*>(ws + RECORD_BYTES + SHARED_BYTES);
     const cudaError_t e = a.add_weights ? launch_split<true>(a, map, s) : launch_split<false>(a, map, s);
-    if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(CTAS); cfg.blockDim = dim3(JOIN_THREADS); cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attn_paged_join_kernel, a);
+    return e != cudaSuccess ? e : launch_dependent(attn_paged_join_kernel, JOIN_THREADS, 0, s, a);
 }
 
 }  // namespace qattn
