@@ -57,7 +57,6 @@ constexpr int STAGES = 3;                     // blocks in flight per warp
 constexpr int HALF_STAGE = BLK * D * 2;       // K rows, then V rows of a block: 4 KB each, [channel half][row][64]
 constexpr int STAGE = 2 * HALF_STAGE;
 constexpr int RING = WARPS * STAGES * STAGE;
-constexpr int Q_WORDS = GROUP * D;            // a warp's query halves, packed (high, low)
 constexpr int CTAS = NUM_SMS_B200;            // ranges
 constexpr int MIN_BLOCKS = WARPS;             // blocks per range, at least
 constexpr int JOIN_THREADS = 256, JOIN_GROUPS = JOIN_THREADS / (GROUP * D / 4);
@@ -82,9 +81,8 @@ __device__ __forceinline__ int row_length(const PagedAttnArgs& a, int b) {
     return paged_length(a.lengths[b], a.cols, a.kv.shift);
 }
 
-// start[b] = blocks of rows [0, b), length[b] its cached rows; called by all threads of the CTA,
-// n <= MAX_PAGED_BATCH.
-__device__ __forceinline__ PagedSplit scan_lengths(const PagedAttnArgs& a, int* start, int* length, int* warp_sum) {
+// start[b] = blocks of rows [0, b); called by all threads of the CTA, n <= MAX_PAGED_BATCH.
+__device__ __forceinline__ PagedSplit scan_lengths(const PagedAttnArgs& a, int* start, int* warp_sum) {
     constexpr int PER = MAX_PAGED_BATCH / THREADS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int v[PER], sum = 0;
@@ -92,11 +90,7 @@ __device__ __forceinline__ PagedSplit scan_lengths(const PagedAttnArgs& a, int* 
     for (int i = 0; i < PER; ++i) {
         const int b = tid * PER + i;
         v[i] = sum;
-        if (b < a.n) {
-            const int len = row_length(a, b);
-            length[b] = len;
-            sum += (len + BLK - 1) / BLK;
-        }
+        if (b < a.n) sum += (row_length(a, b) + BLK - 1) / BLK;
     }
     int incl = sum;
     #pragma unroll
@@ -179,9 +173,8 @@ template <bool WEIGHTS>
 __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap map) {
     extern __shared__ __align__(1024) uint8_t ring[];        // [WARPS][STAGES][K rows | V rows]
     __shared__ __align__(8) uint64_t full[WARPS][STAGES];
-    __shared__ int start[MAX_PAGED_BATCH + 1], length[MAX_PAGED_BATCH];
+    __shared__ int start[MAX_PAGED_BATCH + 1];
     __shared__ int warp_sum[WARPS];
-    __shared__ __align__(16) uint32_t s_q[WARPS][Q_WORDS];
     __shared__ Part parts[WARPS][2];                         // [0]: of the warp's first unit, [1]: of its last
     __shared__ __align__(16) float s_part[WARPS][2][GROUP * D];
     __shared__ int abort_flag, never_abort;
@@ -197,7 +190,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
     if (tid < WARPS * 2) parts[tid >> 1][tid & 1].unit = -1;
     asm volatile("griddepcontrol.wait;" ::: "memory");       // what ran before is complete
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const PagedSplit sp = scan_lengths(a, start, length, warp_sum);   // its barriers publish the above too
+    const PagedSplit sp = scan_lengths(a, start, warp_sum);   // its barriers publish the above too
     if (sp.total == 0 || c >= sp.ctas) {
         if (tid < 2) shared_of(a)[c * 2 + tid].nrec = 0;
         return;
@@ -227,6 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
         auto from_first = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
         u.l = from_first(u.l); u.b = from_first(u.b); u.kh = from_first(u.kh); u.nblk = from_first(u.nblk);
         u.off = __shfl_sync(0xffffffffu, u.off, 0);          // the unit of g_begin
+        const uint64_t once = policy_evict_first();
         int rows_now = place();                              // of the batch being copied
         const int n_blocks = (int)(g_end - g_begin);
         uint32_t valid = 0;                                  // bit per stage: the block was copied
@@ -247,8 +241,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
             __syncwarp();
             if (ok && lane < 4) {                            // lane: K or V, channel half
                 const int kv = lane >> 1, half = lane & 1;
-                tma_load_2d(my_ring + stage * STAGE + kv * HALF_STAGE + half * (HALF_STAGE / 2), &map, half * 64,
-                            row + (kv * hkv << a.kv.shift), &my_full[stage]);
+                tma_load_2d_once(my_ring + stage * STAGE + kv * HALF_STAGE + half * (HALF_STAGE / 2), &map, half * 64,
+                            row + (kv * hkv << a.kv.shift), &my_full[stage], once);
             }
             ++issued;
         };
@@ -266,9 +260,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
         // x ^ (r % 8) of its 128-byte line); K: rows in the low bit of the matrix index, V: chunks
         const int mi = lane >> 3, k_row = (lane & 7) + (mi & 1) * 8, v_row = (lane & 7) + (mi >> 1) * 8;
         const uint32_t ring_addr = smem_u32(my_ring);
+        // a unit's query halves, packed (high, low), go through the slot of the warp's last part, which
+        // is written after that part's queries are in registers
+        uint32_t* const s_q = reinterpret_cast<uint32_t*>(s_part[warp][1]);
         for (long long g = g_begin; g < g_end;) {
             const int cnt = (int)(min(u.off + u.nblk, g_end) - g), blk0 = (int)(g - u.off);
-            const int len = length[u.b];
+            const int len = row_length(a, u.b);
             uint32_t qf[16];                                 // column g8: head (g8 / 2) % 2, its high or low half by g8 % 2
             float unscale;                                   // logit = unscale * dot product, of head `head`
             {
@@ -285,12 +282,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
                 uint32_t h[8];
                 #pragma unroll
                 for (int i = 0; i < 8; ++i) h[i] = split_half(v[i] * scale);
-                uint4* to = reinterpret_cast<uint4*>(&s_q[warp][lane * 8]);
+                uint4* to = reinterpret_cast<uint4*>(s_q + lane * 8);
                 to[0] = make_uint4(h[0], h[1], h[2], h[3]);
                 to[1] = make_uint4(h[4], h[5], h[6], h[7]);
                 __syncwarp();
                 // channels 16 k + 2 j4 + {0, 1} and + {8, 9} of step k
-                const uint2* from = reinterpret_cast<const uint2*>(&s_q[warp][(g8 >> 1 & 1) * D + 2 * j4]);
+                const uint2* from = reinterpret_cast<const uint2*>(s_q + (g8 >> 1 & 1) * D + 2 * j4);
                 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const uint2 x = from[4 * i];
@@ -396,10 +393,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
                 }
                 if (lane < GROUP) { parts[warp][slot].m[lane] = m; parts[warp][slot].l[lane] = l; }
             }
+            const float inv = whole ? 1.f / l : 1.f;
             #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float x = (j4 < 2 ? acc[i][0] + acc[i][1] : acc[i][2] + acc[i][3]);
-                to[head * D + 16 * i + g8 + (j4 < 2 ? 0 : 8)] = whole ? x / l : x;
+                to[head * D + 16 * i + g8 + (j4 < 2 ? 0 : 8)] = x * inv;
             }
             if (WEIGHTS && whole) {
                 const float M[GROUP] = {__shfl_sync(0xffffffffu, m, 0), __shfl_sync(0xffffffffu, m, 1)};
@@ -421,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
     p.unit = -1;
     if (lane < WARPS * 2) p = parts[lane >> 1][lane & 1];
     unsigned left = __ballot_sync(0xffffffffu, p.unit >= 0);
-    bool have[2] = {false, false};                           // records of this range
+    unsigned have = 0;                                       // records of this range
     while (left) {
         const int first = __ffs(left) - 1;
         const int unit = __shfl_sync(0xffffffffu, p.unit, first), blk0 = __shfl_sync(0xffffffffu, p.blk0, first);
@@ -455,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
             a.out[(size_t)unit * GROUP * D + tid] = o / (head1 ? L[1] : L[0]);
             if (WEIGHTS) {
                 const int lb = unit / hkv, row_l = lb / a.n, row_b = lb - row_l * a.n, row_kh = unit - lb * hkv;
-                add_weights(a, row_l, row_b, row_kh, length[row_b], 0, cnt, g, M, L, tid, THREADS);
+                add_weights(a, row_l, row_b, row_kh, row_length(a, row_b), 0, cnt, g, M, L, tid, THREADS);
             }
         } else {
             const int slot = g != c_begin;
@@ -471,15 +469,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
                 s.unit = unit; s.blk0 = blk0; s.cnt = cnt; s.g = g;
                 shared_of(a)[c * 2 + slot] = s;
             }
-            have[slot] = true;
+            have |= 1u << slot;
         }
     }
-    if (tid < 2 && !have[tid]) shared_of(a)[c * 2 + tid].nrec = 0;
+    if (tid < 2 && !(have >> tid & 1)) shared_of(a)[c * 2 + tid].nrec = 0;
 }
 
 // CTA c joins the unit whose first range is c and, with weights, adds those of the parts of shared
 // units that lie in range c. Beside that, before the first launch is done: rows of length 0.
-__global__ void __launch_bounds__(JOIN_THREADS) attn_paged_join_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(JOIN_THREADS, 5) attn_paged_join_kernel(const PagedAttnArgs a) {
     __shared__ float s_f[CTAS][GROUP];                       // factor of each record
     __shared__ float red[2 * GROUP][JOIN_THREADS / 32];
     __shared__ __align__(16) float s_sum[JOIN_GROUPS][GROUP * D];
@@ -537,7 +535,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attn_paged_join_kernel(const Pag
             // four columns a thread, every fourth record a group, then the groups in order
             const int grp = tid / (GROUP * D / 4), col = tid % (GROUP * D / 4) * 4;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            #pragma unroll 8
+            #pragma unroll 4
             for (int i = grp; i < s.nrec; i += JOIN_GROUPS) {
                 const float4 x = *reinterpret_cast<const float4*>((i ? others + (size_t)i * 2 * PARTIAL_FLOATS : first) + 4 + col);
                 const float f = s_f[i][col / D];
