@@ -53,7 +53,7 @@ using namespace sm100;
 
 constexpr int WARPS = 8, THREADS = WARPS * 32;
 constexpr int BLK = PAGED_BLK;
-constexpr int STAGES = 3;                     // blocks in flight per warp
+constexpr int STAGES = 2;                     // blocks in flight per warp
 constexpr int HALF_STAGE = BLK * D * 2;       // K rows, then V rows of a block: 4 KB each, [channel half][row][64]
 constexpr int STAGE = 2 * HALF_STAGE;
 constexpr int RING = WARPS * STAGES * STAGE;
