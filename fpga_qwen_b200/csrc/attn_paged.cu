@@ -414,11 +414,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
     __syncthreads();
 
     // ---- merge the warps' parts: those of one unit are neighbours in the order of the blocks ----
-    // every warp holds all parts, one a lane; thread: column tid of [GROUP][D]
-    Part p;
-    p.unit = -1;
-    if (lane < WARPS * 2) p = parts[lane >> 1][lane & 1];
-    unsigned left = __ballot_sync(0xffffffffu, p.unit >= 0);
+    // every warp holds all parts, two lanes each: lane is part lane % 16 and head lane / 16
+    static_assert(WARPS * 2 == 16, "two heads of all parts fill a warp");
+    const int part = lane & 15, part_head = lane >> 4;
+    const Part p = parts[part >> 1][part & 1];
+    const float p_m = part_head ? p.m[1] : p.m[0], p_l = part_head ? p.l[1] : p.l[0];
+    unsigned left = __ballot_sync(0xffffffffu, p.unit >= 0) & 0xffff;
     unsigned have = 0;                                       // records of this range
     while (left) {
         const int first = __ffs(left) - 1;
@@ -426,27 +427,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
         const int nblk = __shfl_sync(0xffffffffu, p.nblk, first);
         const long long g = __shfl_sync(0xffffffffu, p.g, first);
         const bool mine = p.unit == unit;
-        const unsigned group = __ballot_sync(0xffffffffu, mine);
+        const unsigned group = __ballot_sync(0xffffffffu, mine) & 0xffff;
         left &= ~group;
-        const int cnt = __reduce_add_sync(0xffffffffu, mine ? p.cnt : 0);
-        float M[GROUP], L[GROUP], f[GROUP];
+        const int cnt = __reduce_add_sync(0xffffffffu, mine && part_head == 0 ? p.cnt : 0);
+        float top = mine ? p_m : -INFINITY;
         #pragma unroll
-        for (int k = 0; k < GROUP; ++k) {
-            M[k] = mine ? p.m[k] : -INFINITY;
-            #pragma unroll
-            for (int x = WARPS; x >= 1; x >>= 1) M[k] = fmaxf(M[k], __shfl_xor_sync(0xffffffffu, M[k], x, WARPS * 2));
-            M[k] = __shfl_sync(0xffffffffu, M[k], 0);
-            f[k] = mine ? exp2_from(p.m[k], M[k]) : 0.f;
-            L[k] = mine ? f[k] * p.l[k] : 0.f;
-            #pragma unroll
-            for (int x = WARPS; x >= 1; x >>= 1) L[k] += __shfl_xor_sync(0xffffffffu, L[k], x, WARPS * 2);
-            L[k] = __shfl_sync(0xffffffffu, L[k], 0);
-        }
+        for (int x = 8; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float f = mine ? exp2_from(p_m, top) : 0.f;
+        float sum = mine ? f * p_l : 0.f;
+        #pragma unroll
+        for (int x = 8; x >= 1; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        const float M[GROUP] = {__shfl_sync(0xffffffffu, top, 0), __shfl_sync(0xffffffffu, top, 16)};
+        const float L[GROUP] = {__shfl_sync(0xffffffffu, sum, 0), __shfl_sync(0xffffffffu, sum, 16)};
         const bool head1 = tid >= D;                         // (a warp's columns are of one head)
         float o = 0.f;
         #pragma unroll
         for (int k = 0; k < WARPS * 2; ++k) {
-            const float fk = __shfl_sync(0xffffffffu, head1 ? f[1] : f[0], k);
+            const float fk = __shfl_sync(0xffffffffu, f, k + (head1 ? 16 : 0));
             if (group >> k & 1) o += fk * s_part[k >> 1][k & 1][tid];
         }
         if (cnt == nblk) {
@@ -460,7 +457,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
             float* rec = a.records + ((size_t)c * 2 + slot) * PARTIAL_FLOATS;
             if (tid < GROUP) { rec[tid] = M[tid]; rec[GROUP + tid] = L[tid]; }
             rec[4 + tid] = o;
-            if (tid == 0) {
+            if (tid == slot * 32) {
                 const long long off = g - blk0;
                 Shared s;
                 s.first = sp.range_of(off);
