@@ -4,171 +4,219 @@
 // the L - recent older ones the keep - recent with the largest weights (ties: the lower row; NaN
 // below everything).
 //
-// Selection (one CTA per unit): a radix search of the threshold over order-preserving 32-bit keys,
-// eight bits a pass (histogram, then a parallel scan from its top bin), then one ascending pass
-// that places every kept row: a row's new index is (rows above the threshold before it) +
-// min(tied rows before it, ties to keep), so one scan of both counts serves. Where the table has
-// at most SEL_THREADS * PER rows the weights stay in registers from the first load on; longer
-// caches read them again for each pass (from L2).
+// Selection: a radix search of the threshold over order-preserving 32-bit keys, eight bits a pass,
+// then one ascending pass that places every kept row: a row's new index is (rows above the
+// threshold before it) + min(tied rows before it, ties to keep), so one scan of both counts serves.
+// It is a chain of latencies and of code that runs once, so barriers are few (a histogram per pass,
+// all cleared at the start; every warp scans the bins, and later the counts, for itself) and the
+// code is small: weights lie in shared memory, not in registers, and loops stay rolled. (Unrolled
+// over registers it took 10 us for 8 units of 1025 rows, most of it fetching instructions.
+// Counting two bits at a time without atomics took twice as long as the histograms.) One CTA takes
+// a unit; where the table can hold more than 4096 rows, a cluster of CTAs takes it, each a
+// contiguous slice of its rows, and histograms and counts are summed over distributed shared
+// memory.
 //
-// The move is bound by HBM (512 bytes read and 512 written per kept row) and goes forward in
-// tiles: the j-th kept row's old index is at least j, so a tile's destinations lie at or below
-// every later tile's sources, and a barrier between a tile's loads and its stores makes the move
-// safe in place. Channels are independent: a unit's K or V rows are split over CTAs by channel
-// slice, not by row, and only as far as it takes to fill the GPU (narrow slices cost DRAM
-// efficiency).
+// The move is bound by HBM (512 bytes read and 512 written per kept row; whole rows at a time, since
+// narrow column slices cost DRAM efficiency: 107 us in 64-byte and 154 us in 32-byte slices against
+// 88 us in whole rows, for 2048 rows x 224 units). It goes forward in tiles: the j-th kept row's
+// old index is at least j, so a tile's destinations lie at or below every later tile's sources,
+// and a barrier between a tile's loads and its stores makes the move safe in place. A unit's K
+// or V rows are moved by one CTA, or by a cluster where there are few units, whose CTAs each take
+// a part of every tile and meet at the cluster's barrier.
+#include <cooperative_groups.h>
+
 #include "qattn_common.cuh"
 
 namespace qattn {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32;
-constexpr int BINS = 256;
+constexpr int BINS = 256, BATCH = 8;
+constexpr int SLICE_ROWS = 4096;                   // of a cluster's CTA, where there are SMs for it
+constexpr int MAX_SLICE = 49152;                   // 192 KB of shared memory
+constexpr int TABLE_INTS = 1024;                   // page ids of the destination kept in shared memory
 
 __device__ __forceinline__ int row_length(const PagedEvictArgs& a, int b) {
     return paged_length(a.lengths[b], a.src_cols, a.kv.shift);
 }
 
-// The thread's rows are tid, tid + SEL_THREADS, ...: PER of them, held in registers (CACHED), or
-// as many as there are, in tiles of PER.
-template <int PER, bool CACHED>
+// The cluster's CTAs each take a contiguous slice of the unit's rows, at most as many as s_w holds.
 __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const PagedEvictArgs a) {
-    __shared__ int hist[BINS];
-    __shared__ int s_scan[BINS / 32], s_bin, s_need;
-    __shared__ int s_cnt[PER * SEL_WARPS], s_off[PER * SEL_WARPS + 1];
-    static_assert(PER * SEL_WARPS <= SEL_THREADS && PER * SEL_WARPS % 32 == 0, "one scan over the tile's warps");
+    extern __shared__ __align__(16) float s_w[];             // the slice's weights
+    __shared__ __align__(16) int hist[4][BINS];
+    __shared__ __align__(16) int bins[2][BINS];              // of the whole cluster, by turns
+    __shared__ int s_dst[TABLE_INTS];
+    __shared__ int s_cnt[SEL_WARPS], s_total;                // packed counts: above the threshold, tied << 16
+    cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int h = blockIdx.x % a.kv.hkv, layer = (blockIdx.x / a.kv.hkv) % a.kv.layers, b = blockIdx.x / (a.kv.hkv * a.kv.layers);
+    const int rank = cluster.block_rank(), ranks = cluster.num_blocks();
+    const int unit = blockIdx.x / ranks;
+    const int h = unit % a.kv.hkv, layer = (unit / a.kv.hkv) % a.kv.layers, b = unit / (a.kv.hkv * a.kv.layers);
     const int L = row_length(a, b), mask = (1 << a.kv.shift) - 1;
-    if (tid == 0 && a.lengths[b] != L) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
-    int* kept = a.kept + (size_t)blockIdx.x * a.keep;
+    int* kept = a.kept + (size_t)unit * a.keep;
     const int* src = a.src_table + (size_t)b * a.src_cols;
     const int* dst = a.dst_table + (size_t)b * a.dst_cols;
     const bool all = L <= a.keep;
-    const int old = L - a.recent;                  // rows that compete (unless all stay)
+    const int old = all ? 0 : L - a.recent;                  // rows that compete
+    const int per = (L + ranks - 1) / ranks;
+    const int row0 = min(rank * per, L), rows = min(L - row0, per), compete = min(max(old - row0, 0), rows);
 
-    float w[PER];
-    auto load_tile = [&](int t0) {
-        int page[PER];
+    for (int i = tid; i < 4 * BINS; i += SEL_THREADS) hist[0][i] = 0;
+    const int dst_used = ((a.keep - 1) >> a.kv.shift) + 1;
+    if (dst_used <= TABLE_INTS) {
+        for (int i = tid; i < dst_used; i += SEL_THREADS) s_dst[i] = __ldg(dst + i);
+        dst = s_dst;
+    }
+    if (tid == 0 && rank == 0 && a.lengths[b] != L) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
+    #pragma unroll 1
+    for (int i0 = tid; i0 < rows; i0 += SEL_THREADS * BATCH) {
+        // all page ids of a batch, then all its weights, in flight at once
+        int page[BATCH];
+        float w[BATCH];
         #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int t = t0 + i * SEL_THREADS + tid;
-            page[i] = t < L ? src[t >> a.kv.shift] : -1;
+        for (int k = 0; k < BATCH; ++k) {
+            const int i = i0 + k * SEL_THREADS;
+            page[k] = i < rows ? __ldg(src + ((row0 + i) >> a.kv.shift)) : 0;
         }
+        int bad = 0;
         #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int t = t0 + i * SEL_THREADS + tid;
-            w[i] = 0.f;
-            if (a.kv.has(page[i])) w[i] = *a.kv.weight(page[i], layer, h, t & mask);
-            else if (t < L) atomicCAS(a.error, 0, PAGED_BAD_PAGE);
+        for (int k = 0; k < BATCH; ++k) {
+            const int i = i0 + k * SEL_THREADS;
+            const bool ok = a.kv.has(page[k]);
+            bad |= !ok;
+            w[k] = ok && i < rows ? *a.kv.weight(page[k], layer, h, (row0 + i) & mask) : 0.f;
         }
-    };
-    if (CACHED) load_tile(0);
+        if (bad) atomicCAS(a.error, 0, PAGED_BAD_PAGE);
+        #pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+            if (i0 + k * SEL_THREADS < rows) s_w[i0 + k * SEL_THREADS] = w[k];
+    }
+    __syncthreads();
+    // prefix: the threshold, the key of rank `need`; need: first the competing rows to keep, then those
+    // of them equal to the threshold
     unsigned prefix = 0;
-    int need = a.keep - a.recent;                  // competing rows to keep
-    if (!all && need > 0) {
-        // threshold: the key of rank `need`; need becomes the number of rows equal to it to keep
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < BINS) hist[tid] = 0;
-            __syncthreads();
-            for (int t0 = 0; t0 < old; t0 += SEL_THREADS * PER) {
-                if (!CACHED) load_tile(t0);
-                #pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    const unsigned k = evict_key(w[i]);
-                    if (t0 + i * SEL_THREADS + tid < old && (shift == 24 || ((k ^ prefix) >> (shift + 8)) == 0))
-                        atomicAdd(&hist[(k >> shift) & (BINS - 1)], 1);
-                }
-            }
-            __syncthreads();
-            // thread i: bin BINS - 1 - i; the bin whose count from the top reaches `need`
-            int mine = 0, incl = 0;
-            if (tid < BINS) {
-                mine = incl = hist[BINS - 1 - tid];
-                #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int x = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += x;
-                }
-                if (lane == 31) s_scan[warp] = incl;
-            }
-            __syncthreads();
-            if (tid < BINS) {
-                for (int x = 0; x < warp; ++x) incl += s_scan[x];
-                if (incl >= need && incl - mine < need) { s_bin = BINS - 1 - tid; s_need = need - (incl - mine); }
-            }
-            __syncthreads();
-            prefix |= (unsigned)s_bin << shift;
-            need = s_need;
+    int need = all ? 0 : a.keep - a.recent;
+    const bool wanted = need > 0;
+    #pragma unroll 1
+    for (int pass = 0; pass < 4 && wanted; ++pass) {
+        const int shift = 24 - 8 * pass;
+        const unsigned known = pass ? ~0u << (shift + 8) : 0u;
+        #pragma unroll 4
+        for (int i = tid; i < compete; i += SEL_THREADS) {
+            const unsigned k = evict_key(s_w[i]);
+            if (((k ^ prefix) & known) == 0) atomicAdd(&hist[pass][(k >> shift) & (BINS - 1)], 1);
         }
-    }
-    // ---- ascending pass: indices and weights of the kept rows ----
-    int above0 = 0, ties0 = 0;                     // rows above the threshold, and tied with it, before this tile
-    for (int t0 = 0; t0 < L; t0 += SEL_THREADS * PER) {
-        if (!CACHED) load_tile(t0);
-        unsigned up[PER], tie[PER];                // ballots of the warp
-        #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int t = t0 + i * SEL_THREADS + tid;
-            const unsigned k = evict_key(w[i]);
-            const bool competes = t < old && !all, wanted = a.keep > a.recent;
-            up[i] = __ballot_sync(0xffffffffu, t < L && (competes ? wanted && k > prefix : true));
-            tie[i] = __ballot_sync(0xffffffffu, competes && wanted && k == prefix);
-            if (lane == 0) s_cnt[i * SEL_WARPS + warp] = __popc(up[i]) | __popc(tie[i]) << 16;   // at most 8192 each
-        }
-        __syncthreads();                           // every load of the tile is done too: the stores below may overlap it
-        // exclusive scan of the PER * SEL_WARPS packed counts, in row order
-        int mine = 0, incl = 0;
-        if (tid < PER * SEL_WARPS) {
-            mine = incl = s_cnt[tid];
-            #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += x;
+        const int* total = hist[pass];
+        if (ranks > 1) {
+            cluster.sync();
+            if (tid < BINS) {
+                int sum = 0;
+                #pragma unroll 4
+                for (int r = 0; r < ranks; ++r) sum += cluster.map_shared_rank(hist[pass], r)[tid];
+                bins[pass & 1][tid] = sum;
             }
-            if (lane == 31) s_scan[warp] = incl;
+            total = bins[pass & 1];
         }
         __syncthreads();
-        if (tid < PER * SEL_WARPS) {
-            for (int x = 0; x < warp; ++x) incl += s_scan[x];
-            s_off[tid] = incl - mine;
-            if (tid == PER * SEL_WARPS - 1) s_off[PER * SEL_WARPS] = incl;
-        }
-        __syncthreads();
+        // lane: bins 255 - 8 lane down to 248 - 8 lane; the bin whose count from the top reaches `need`
+        const int4 hi = *reinterpret_cast<const int4*>(total + BINS - 4 - 8 * lane);
+        const int4 lo = *reinterpret_cast<const int4*>(total + BINS - 8 - 8 * lane);
+        const int v[8] = {hi.w, hi.z, hi.y, hi.x, lo.w, lo.z, lo.y, lo.x};
+        int sum = 0;
         #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int t = t0 + i * SEL_THREADS + tid, off = s_off[i * SEL_WARPS + warp];
-            const unsigned before = (1u << lane) - 1u;
-            const int ties = ties0 + (off >> 16) + __popc(tie[i] & before);
-            const int j = above0 + (off & 0xffff) + __popc(up[i] & before) + min(ties, need);
-            if ((up[i] >> lane & 1) || ((tie[i] >> lane & 1) && ties < need)) {
-                kept[j] = t;
-                const int page = dst[j >> a.kv.shift];
-                if (a.kv.has(page)) *a.kv.weight(page, layer, h, j & mask) = w[i];
-                else atomicCAS(a.error, 0, PAGED_BAD_PAGE);
-            }
+        for (int i = 0; i < 8; ++i) sum += v[i];
+        int incl = sum;
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
         }
-        above0 += s_off[PER * SEL_WARPS] & 0xffff;
-        ties0 += s_off[PER * SEL_WARPS] >> 16;
+        const int at = __ffs(__ballot_sync(0xffffffffu, incl >= need)) - 1;
+        int before = incl - sum, bin = BINS - 1 - 8 * lane;
+        bool found = false;
+        #pragma unroll
+        for (int i = 0; i < 7; ++i) {
+            found = found || before + v[i] >= need;
+            if (!found) { before += v[i]; --bin; }
+        }
+        prefix |= (unsigned)__shfl_sync(0xffffffffu, bin, at) << shift;
+        need -= __shfl_sync(0xffffffffu, before, at);
     }
-    for (int j = above0 + min(ties0, need) + tid; j < a.keep; j += SEL_THREADS) kept[j] = -1;
+    // ---- ascending pass: each warp takes a run of the slice's rows; first it counts ----
+    const int run = ((rows + SEL_WARPS - 1) / SEL_WARPS + 31) & ~31;
+    const int i0 = min(warp * run, rows), i1 = min(i0 + run, rows);
+    auto ballots = [&](int i, unsigned& up, unsigned& tie) {
+        const unsigned k = i < compete ? evict_key(s_w[i]) : 0u;
+        up = __ballot_sync(0xffffffffu, i < i1 && (i < compete ? wanted && k > prefix : true));
+        tie = __ballot_sync(0xffffffffu, i < i1 && i < compete && wanted && k == prefix);
+    };
+    int above = 0, ties = 0;
+    #pragma unroll 2
+    for (int i = i0 + lane; i - lane < i1; i += 32) {
+        unsigned up, tie;
+        ballots(i, up, tie);
+        above += __popc(up);
+        ties += __popc(tie);
+    }
+    // (a slice holds fewer than 2^16 rows, so both counts fit one word)
+    if (lane == 0) s_cnt[warp] = above | ties << 16;
+    __syncthreads();
+    const int c = lane < SEL_WARPS ? s_cnt[lane] : 0, earlier = lane < warp ? c : 0;
+    above = __reduce_add_sync(0xffffffffu, earlier & 0xffff);
+    ties = __reduce_add_sync(0xffffffffu, (unsigned)earlier >> 16);
+    int all_above = __reduce_add_sync(0xffffffffu, c & 0xffff), all_ties = __reduce_add_sync(0xffffffffu, (unsigned)c >> 16);
+    if (ranks > 1) {
+        // the slices before this one; this barrier also follows every CTA's loads of weights
+        if (tid == 0) s_total = all_above | all_ties << 16;
+        cluster.sync();
+        const int t = lane < rank ? *cluster.map_shared_rank(&s_total, lane) : 0;
+        const int above0 = __reduce_add_sync(0xffffffffu, t & 0xffff), ties0 = __reduce_add_sync(0xffffffffu, (unsigned)t >> 16);
+        above += above0; ties += ties0;
+        all_above += above0; all_ties += ties0;
+    }
+    // ---- then it places them ----
+    #pragma unroll 2
+    for (int i = i0 + lane; i - lane < i1; i += 32) {
+        unsigned up, tie;
+        ballots(i, up, tie);
+        const unsigned before = (1u << lane) - 1u;
+        const int my_ties = ties + __popc(tie & before);
+        const int j = above + __popc(up & before) + min(my_ties, need);
+        if ((up >> lane & 1) || ((tie >> lane & 1) && my_ties < need)) {
+            kept[j] = row0 + i;
+            const int page = dst[j >> a.kv.shift];
+            if (a.kv.has(page)) *a.kv.weight(page, layer, h, j & mask) = s_w[i];
+            else atomicCAS(a.error, 0, PAGED_BAD_PAGE);
+        }
+        above += __popc(up);
+        ties += __popc(tie);
+    }
+    if (rank == ranks - 1)                                   // (the last slice's counts are the unit's)
+        for (int j = all_above + min(all_ties, need) + tid; j < a.keep; j += SEL_THREADS) kept[j] = -1;
+    if (ranks > 1) cluster.sync();                           // until the others have read this CTA's memory
 }
 
 constexpr int MOVE_THREADS = 256, UNROLL = 4;
+constexpr int MOVE_ROWS = MOVE_THREADS / 16;       // rows per load: 16 threads of 16 bytes each
 
-// CTA (unit, K|V, channel slice of SLICE 16-byte chunks): moves the kept rows' slices.
-template <int SLICE>
+// Cluster (unit, K|V): moves the kept rows, tile after tile of UNROLL * MOVE_ROWS rows per CTA. Three
+// tiles are under way: one being stored, the next one's rows and the one after's indices and
+// pages being loaded. A tile's rows may be loaded before the tile before it is stored, since its
+// sources lie above those destinations.
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const PagedEvictArgs a) {
-    constexpr int ROWS = MOVE_THREADS / SLICE;     // rows per load
-    const int unit = blockIdx.x, kv = blockIdx.y, slice = blockIdx.z;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const int unit = blockIdx.x / ranks, kv = blockIdx.y, tile = UNROLL * MOVE_ROWS * ranks;
     const int h = unit % a.kv.hkv, layer = (unit / a.kv.hkv) % a.kv.layers, b = unit / (a.kv.hkv * a.kv.layers);
     const int mask = (1 << a.kv.shift) - 1;
-    const int chunk = slice * SLICE + threadIdx.x % SLICE, r = threadIdx.x / SLICE;
+    const int chunk = threadIdx.x & 15, r = rank * (UNROLL * MOVE_ROWS) + (threadIdx.x >> 4);
     const int* kept = a.kept + (size_t)unit * a.keep;
     const int* src = a.src_table + (size_t)b * a.src_cols;
     const int* dst = a.dst_table + (size_t)b * a.dst_cols;
     asm volatile("griddepcontrol.wait;" ::: "memory");       // the selection is complete
-    if (layer == 0 && h == 0 && kv == 0 && slice == 0 && threadIdx.x == 0) {
+    if (layer == 0 && h == 0 && kv == 0 && rank == 0 && threadIdx.x == 0) {
         int lo = 0, hi = a.keep;                   // kept rows: the first -1
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
@@ -176,40 +224,67 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const PagedEvi
         }
         a.new_lengths[b] = lo;
     }
-    for (int j0 = 0; j0 < a.keep; j0 += ROWS * UNROLL) {
-        uint4 v[UNROLL];
-        int from[UNROLL], to[UNROLL];
+    int from[UNROLL], page[UNROLL], to[UNROLL];    // of the tile ahead: old row, its page, the new row's page (-1: no move)
+    auto load_index = [&](int j0) {
         #pragma unroll
         for (int i = 0; i < UNROLL; ++i) {
-            const int j = j0 + i * ROWS + r;
-            from[i] = j < a.keep ? kept[j] : -1;
+            const int j = j0 + i * MOVE_ROWS + r;
+            from[i] = j < a.keep ? __ldg(kept + j) : -1;
         }
+    };
+    auto load_pages = [&](int j0) {
         #pragma unroll
         for (int i = 0; i < UNROLL; ++i) {
-            const int j = j0 + i * ROWS + r;
-            const int page = from[i] < 0 ? -1 : src[from[i] >> a.kv.shift];
-            to[i] = from[i] < 0 ? -1 : dst[j >> a.kv.shift];
-            if (!a.kv.has(page)) to[i] = -1;       // recorded by the selection
-            else v[i] = reinterpret_cast<const uint4*>(a.kv.row(page, layer, kv, h, from[i] & mask))[chunk];
+            const int j = j0 + i * MOVE_ROWS + r;
+            page[i] = from[i] < 0 ? -1 : __ldg(src + (from[i] >> a.kv.shift));
+            to[i] = from[i] < 0 ? -1 : __ldg(dst + (j >> a.kv.shift));
         }
-        __syncthreads();
+    };
+    uint4 v[UNROLL], next[UNROLL];
+    int dest[UNROLL], next_dest[UNROLL];           // page to store to, or -1
+    auto load_rows = [&](uint4 (&x)[UNROLL], int (&d)[UNROLL]) {
         #pragma unroll
         for (int i = 0; i < UNROLL; ++i) {
-            const int j = j0 + i * ROWS + r;
-            if (a.kv.has(to[i])) reinterpret_cast<uint4*>(a.kv.row(to[i], layer, kv, h, j & mask))[chunk] = v[i];
+            d[i] = a.kv.has(page[i]) && a.kv.has(to[i]) ? to[i] : -1;      // (bad pages are recorded by the selection)
+            if (d[i] >= 0) x[i] = reinterpret_cast<const uint4*>(a.kv.row(page[i], layer, kv, h, from[i] & mask))[chunk];
         }
+    };
+    load_index(0);
+    load_pages(0);
+    load_rows(v, dest);
+    load_index(tile);
+    load_pages(tile);
+    for (int j0 = 0; j0 < a.keep; j0 += tile) {
+        load_rows(next, next_dest);                // the tile after this one
+        load_index(min(j0 + 2 * tile, a.keep));
+        if (ranks > 1) cluster.sync(); else __syncthreads();   // every thread has its rows of this tile
+        #pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            const int j = j0 + i * MOVE_ROWS + r;
+            if (dest[i] >= 0) reinterpret_cast<uint4*>(a.kv.row(dest[i], layer, kv, h, j & mask))[chunk] = v[i];
+            v[i] = next[i];
+            dest[i] = next_dest[i];
+        }
+        load_pages(j0 + 2 * tile);
     }
 }
 
-template <int SLICE>
-cudaError_t launch_move(const PagedEvictArgs& a, int units, cudaStream_t s) {
+cudaError_t launch(void (*kernel)(PagedEvictArgs), dim3 grid, int threads, size_t smem, int cluster, bool dependent,
+                   const PagedEvictArgs& a, cudaStream_t s) {
+    cudaError_t e = cudaSuccess;
+    if (smem > 32 << 10) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    if (cluster > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(units, 2, D * 2 / 16 / SLICE); cfg.blockDim = dim3(MOVE_THREADS); cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, evict_move_kernel<SLICE>, a);
+    cfg.gridDim = dim3(grid.x * cluster, grid.y); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cfg.attrs = attr; cfg.numAttrs = dependent ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 }  // namespace
@@ -217,14 +292,21 @@ cudaError_t launch_move(const PagedEvictArgs& a, int units, cudaStream_t s) {
 cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t s) {
     const int units = a.n * a.kv.layers * a.kv.hkv;
     const int max_rows = a.src_cols << a.kv.shift;
-    if (max_rows <= SEL_THREADS * 2) evict_select_kernel<2, true><<<units, SEL_THREADS, 0, s>>>(a);
-    else if (max_rows <= SEL_THREADS * 8) evict_select_kernel<8, true><<<units, SEL_THREADS, 0, s>>>(a);
-    else evict_select_kernel<8, false><<<units, SEL_THREADS, 0, s>>>(a);
-    const cudaError_t e = cudaPeekAtLastError();
+    // selection: clusters that bring a slice down to SLICE_ROWS while all of them fit the GPU at once,
+    // and in any case to what shared memory holds
+    int ranks = 1;
+    while (ranks < 16 && max_rows > ranks * SLICE_ROWS &&
+           (units * ranks * 2 <= 2 * NUM_SMS_B200 || max_rows > ranks * MAX_SLICE))
+        ranks *= 2;
+    const int per = (max_rows + ranks - 1) / ranks;
+    if (per > MAX_SLICE) return cudaErrorInvalidValue;       // (refused before)
+    const cudaError_t e = launch(evict_select_kernel, dim3(units), SEL_THREADS, (size_t)per * sizeof(float), ranks, false, a, s);
     if (e != cudaSuccess) return e;
-    if (units >= 2 * NUM_SMS_B200) return launch_move<16>(a, units, s);
-    if (units >= NUM_SMS_B200 / 2) return launch_move<8>(a, units, s);
-    return launch_move<2>(a, units, s);
+    // move: clusters that fill the GPU (4 CTAs per SM) where the units alone do not and there are rows
+    // for every CTA
+    ranks = 1;
+    while (ranks < 16 && units * 2 * ranks * 2 <= 4 * NUM_SMS_B200 && ranks * UNROLL * MOVE_ROWS < a.keep) ranks *= 2;
+    return launch(evict_move_kernel, dim3(units, 2), MOVE_THREADS, 0, ranks, true, a, s);
 }
 
 }  // namespace qattn

@@ -1652,6 +1652,8 @@ int qa_paged_evict(qa_ctx* ctx, const qa_pages* pages, const int* src_table, int
         (st = check_ints(ctx, lengths, "lengths")) || (st = check_ints(ctx, new_lengths, "new_lengths")) ||
         (st = check_ints(ctx, kept, "kept")))
         return st;
+    if (src_cols > QA_MAX_EVICT_ROWS / pages->page_rows)
+        return fail(ctx, QA_ERR_INVALID, "source table of %d columns (1..%d)", src_cols, QA_MAX_EVICT_ROWS / pages->page_rows);
     if (keep < 1 || keep > dst_cols * pages->page_rows)
         return fail(ctx, QA_ERR_INVALID, "keep %d rows (1..%d)", keep, dst_cols * pages->page_rows);
     if (recent < 0 || recent > keep) return fail(ctx, QA_ERR_INVALID, "recent %d outside [0,%d]", recent, keep);

@@ -267,6 +267,7 @@ typedef struct qa_pages {
 
 #define QA_MAX_PAGED_BATCH 1024       /* sequences of one attention or eviction call */
 #define QA_MAX_PAGED_ROWS (1 << 20)   /* cache rows of one sequence, new rows of one append, RoPE positions */
+#define QA_MAX_EVICT_ROWS (1 << 19)   /* cache rows of a sequence that qa_paged_evict takes */
 
 /* Extends the RoPE tables to positions [0, n) (at creation: the context's `context` positions;
  * never shrinks). Rows of a paged cache may sit at any such position, since an eviction shortens
@@ -318,8 +319,8 @@ int qa_paged_attn(qa_ctx* ctx, const qa_pages* pages, const int* table, int tabl
  * sequences share a dst page; in place, src pages are not shared either. new_lengths[b] =
  * min(lengths[b], keep). kept: device, [n][n_layers][hkv_local][keep] ints, receives each kept
  * row's old index (ascending; -1 past new_lengths[b]). Rows of dst pages past new_lengths[b] are
- * left as they were. keep >= 1, 0 <= recent <= keep, keep <= dst_cols * page_rows;
- * 1 <= n <= QA_MAX_PAGED_BATCH. Asynchronous on the context stream. */
+ * left as they were. keep >= 1, 0 <= recent <= keep, keep <= dst_cols * page_rows,
+ * src_cols * page_rows <= QA_MAX_EVICT_ROWS; 1 <= n <= QA_MAX_PAGED_BATCH. Asynchronous on the context stream. */
 int qa_paged_evict(qa_ctx* ctx, const qa_pages* pages, const int* src_table, int src_cols, const int* dst_table,
                    int dst_cols, const int* lengths, int* new_lengths, int n, int keep, int recent, int* kept);
 
