@@ -71,9 +71,28 @@ __global__ void __launch_bounds__(TPB * 4 * HKV) kv_append_kernel(const AppendAr
         const int tb = row / R, r = row - tb * R;
         const int kind = r < HQ ? 0 : (r < HQ + HKV ? 1 : 2);
         if (tb < ntok && kind < 2) {
-            const float* slot = &slots[tb * SLOT];
             float* x = &tile[row * STRIDE];
-            norm_rope_row(x, slot + 128 + kind * D, slot, slot + 64, rms_inv(x, a.eps));
+            const float* slot = &slots[tb * SLOT];
+            const float* cs = slot;
+            const float* sn = slot + 64;
+            const float* w = slot + 128 + kind * D;
+            const float inv = rms_inv(x, a.eps);
+            #pragma unroll 4
+            for (int j = 0; j < 64; j += 4) {
+                const float4 xa = *reinterpret_cast<const float4*>(x + j);
+                const float4 xb = *reinterpret_cast<const float4*>(x + j + 64);
+                const float4 wa = *reinterpret_cast<const float4*>(w + j);
+                const float4 wb = *reinterpret_cast<const float4*>(w + j + 64);
+                const float4 c = *reinterpret_cast<const float4*>(cs + j);
+                const float4 s = *reinterpret_cast<const float4*>(sn + j);
+                float ra[4], rb[4];
+                norm_rope_pair(xa.x, xb.x, wa.x, wb.x, c.x, s.x, inv, ra[0], rb[0]);
+                norm_rope_pair(xa.y, xb.y, wa.y, wb.y, c.y, s.y, inv, ra[1], rb[1]);
+                norm_rope_pair(xa.z, xb.z, wa.z, wb.z, c.z, s.z, inv, ra[2], rb[2]);
+                norm_rope_pair(xa.w, xb.w, wa.w, wb.w, c.w, s.w, inv, ra[3], rb[3]);
+                *reinterpret_cast<float4*>(x + j) = make_float4(ra[0], ra[1], ra[2], ra[3]);
+                *reinterpret_cast<float4*>(x + j + 64) = make_float4(rb[0], rb[1], rb[2], rb[3]);
+            }
         }
     }
     __syncthreads();
@@ -88,9 +107,16 @@ __global__ void __launch_bounds__(TPB * 4 * HKV) kv_append_kernel(const AppendAr
         } else if (lane < 16) {
             const int kind = r < HQ + HKV ? 1 : 2;
             const int head = kind == 1 ? r - HQ : r - HQ - HKV;
+            const float4 lo = *reinterpret_cast<const float4*>(x + lane * 8);
+            const float4 hi = *reinterpret_cast<const float4*>(x + lane * 8 + 4);
+            __half2 h0 = __floats2half2_rn(lo.x, lo.y), h1 = __floats2half2_rn(lo.z, lo.w);
+            __half2 h2 = __floats2half2_rn(hi.x, hi.y), h3 = __floats2half2_rn(hi.z, hi.w);
+            uint4 packed;
+            packed.x = *reinterpret_cast<uint32_t*>(&h0); packed.y = *reinterpret_cast<uint32_t*>(&h1);
+            packed.z = *reinterpret_cast<uint32_t*>(&h2); packed.w = *reinterpret_cast<uint32_t*>(&h3);
             __half* dst = a.kv.plane(a.rows.seq_of(b0 + tb, a.seq), a.layer0 + l, kind - 1, head) +
                           (size_t)a.rows.pos_of(b0 + tb, a.pos0) * D;
-            reinterpret_cast<uint4*>(dst)[lane] = half8_rn(x + lane * 8);
+            reinterpret_cast<uint4*>(dst)[lane] = packed;
         }
     }
 }

@@ -38,31 +38,8 @@ __device__ __forceinline__ void norm_rope_pair(float xa, float xb, float wa, flo
     rb = __fadd_rn(__fmul_rn(nb, c), __fmul_rn(na, s));
 }
 
-// One staged row x[0..127] in place: norm with inv and weights w, rotation by cs[64], sn[64]
-// (16-byte aligned shared memory).
-__device__ __forceinline__ void norm_rope_row(float* x, const float* w, const float* cs, const float* sn, float inv) {
-    #pragma unroll 4
-    for (int j = 0; j < 64; j += 4) {
-        const float4 xa = *reinterpret_cast<const float4*>(x + j);
-        const float4 xb = *reinterpret_cast<const float4*>(x + j + 64);
-        const float4 wa = *reinterpret_cast<const float4*>(w + j);
-        const float4 wb = *reinterpret_cast<const float4*>(w + j + 64);
-        const float4 c = *reinterpret_cast<const float4*>(cs + j);
-        const float4 s = *reinterpret_cast<const float4*>(sn + j);
-        float ra[4], rb[4];
-        norm_rope_pair(xa.x, xb.x, wa.x, wb.x, c.x, s.x, inv, ra[0], rb[0]);
-        norm_rope_pair(xa.y, xb.y, wa.y, wb.y, c.y, s.y, inv, ra[1], rb[1]);
-        norm_rope_pair(xa.z, xb.z, wa.z, wb.z, c.z, s.z, inv, ra[2], rb[2]);
-        norm_rope_pair(xa.w, xb.w, wa.w, wb.w, c.w, s.w, inv, ra[3], rb[3]);
-        *reinterpret_cast<float4*>(x + j) = make_float4(ra[0], ra[1], ra[2], ra[3]);
-        *reinterpret_cast<float4*>(x + j + 64) = make_float4(rb[0], rb[1], rb[2], rb[3]);
-    }
-}
-
 // Eight consecutive FP32 values as FP16 (round to nearest even), packed for one 16-byte store.
-__device__ __forceinline__ uint4 half8_rn(const float* x) {
-    const float4 lo = *reinterpret_cast<const float4*>(x);
-    const float4 hi = *reinterpret_cast<const float4*>(x + 4);
+__device__ __forceinline__ uint4 half8_rn(const float4& lo, const float4& hi) {
     __half2 h0 = __floats2half2_rn(lo.x, lo.y), h1 = __floats2half2_rn(lo.z, lo.w);
     __half2 h2 = __floats2half2_rn(hi.x, hi.y), h3 = __floats2half2_rn(hi.z, hi.w);
     uint4 packed;
