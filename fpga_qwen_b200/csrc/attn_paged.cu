@@ -24,7 +24,9 @@
 // Numerics: FP16 rows are exact operands. A query (scaled by a power of two so that its largest
 // channel lies in [2^13, 2^14)) and a weight (exp2 of the distance to the maximum, plus 14) are
 // each the sum of two FP16 halves: 22 bits, or 2^-38 of the largest, whichever is coarser; sums are
-// FP32. The high half is rounded towards zero and neither half of a nonzero value is zero, so
+// FP32, and long sums are made by FADD: the tensor core's own accumulation truncates, which over the
+// hundred blocks of a long history costs a few 2^-20 (2.0e-6 off in 2-norm against 64 bits at
+// 131071 rows), so it takes no more than two steps of a chain. The high half is rounded towards zero and neither half of a nonzero value is zero, so
 // both have its sign and an infinite key or value gives what the formula gives.
 //
 // A unit that several warps of a CTA share is merged through shared memory at the CTA's end; a
@@ -153,6 +155,12 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d = a b.
+__device__ __forceinline__ void mma16816_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // x, |x| < 65504, as high + low FP16 halves (high in the low 16 bits). High is x towards zero; the
@@ -315,16 +323,17 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
                 if (got && (valid >> stage & 1)) {
                     const uint32_t k_addr = ring_addr + stage * STAGE + k_row * 128, v_addr = ring_addr + stage * STAGE + HALF_STAGE + v_row * 128;
                     // logits: rows g8 and g8 + 8 of the block, columns 2 j4 (high) and 2 j4 + 1 (low)
-                    float sc[2][4] = {};
+                    float sc[4][4];
                     #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         uint32_t kf[4];
                         const int chunk = (2 * k + (mi >> 1)) & 7;
                         ldmatrix4(kf, k_addr + (k >> 2) * (HALF_STAGE / 2) + ((chunk ^ (k_row & 7)) << 4));
-                        mma16816(sc[k & 1], kf, qf[2 * k], qf[2 * k + 1]);
+                        if (k < 4) mma16816_new(sc[k], kf, qf[2 * k], qf[2 * k + 1]);
+                        else mma16816(sc[k - 4], kf, qf[2 * k], qf[2 * k + 1]);
                     }
-                    float s0 = ((sc[0][0] + sc[1][0]) + (sc[0][1] + sc[1][1])) * unscale;
-                    float s1 = ((sc[0][2] + sc[1][2]) + (sc[0][3] + sc[1][3])) * unscale;
+                    float s0 = (((sc[0][0] + sc[1][0]) + (sc[2][0] + sc[3][0])) + ((sc[0][1] + sc[1][1]) + (sc[2][1] + sc[3][1]))) * unscale;
+                    float s1 = (((sc[0][2] + sc[1][2]) + (sc[2][2] + sc[3][2])) + ((sc[0][3] + sc[1][3]) + (sc[2][3] + sc[3][3]))) * unscale;
                     if (rows < BLK) {
                         // rows past the length: no logit, and zero V rows, whatever their page holds
                         if (g8 >= rows) s0 = -INFINITY;
@@ -369,7 +378,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
                         uint32_t vf[4];
                         const int chunk = (2 * i + (mi & 1)) & 7;
                         ldmatrix4_trans(vf, v_addr + (i >> 2) * (HALF_STAGE / 2) + ((chunk ^ (v_row & 7)) << 4));
-                        mma16816(acc[i], vf, b0, b1);
+                        float pv[4];
+                        mma16816_new(pv, vf, b0, b1);
+                        #pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][e] += pv[e];
                     }
                 }
                 __syncwarp();                                // the stage is read by all lanes
