@@ -15,6 +15,7 @@
 #include <cstring>
 #include <new>
 #include <string>
+#include <thread>
 #include <vector>
 
 #include "../../include/qattn.h"
@@ -368,12 +369,28 @@ int make_rope_tables(qa_ctx* ctx, int n) {
     }
     double base[64];
     for (int j = 0; j < 64; ++j) base[j] = std::pow(ctx->cfg.rope_theta, 2.0 * j / D);
-    for (int p = 0; p < n; ++p)
-        for (int j = 0; j < 64; ++j) {
-            const double angle = p / base[j];
-            cs[(size_t)p * 64 + j] = (float)std::cos(angle);
-            sn[(size_t)p * 64 + j] = (float)std::sin(angle);
-        }
+    auto fill = [&](int p0, int p1) {
+        for (int p = p0; p < p1; ++p)
+            for (int j = 0; j < 64; ++j) {
+                const double angle = p / base[j];
+                cs[(size_t)p * 64 + j] = (float)std::cos(angle);
+                sn[(size_t)p * 64 + j] = (float)std::sin(angle);
+            }
+    };
+    // long tables on a few host threads (32768 positions: 37 ms on one); what no thread could be
+    // started for is filled here
+    const int parts = n >= 2048 ? (int)std::min(16u, std::max(1u, std::thread::hardware_concurrency())) : 1;
+    const auto edge = [&](int i) { return (int)((long long)n * i / parts); };
+    std::vector<std::thread> threads;
+    int started = 1;
+    try {
+        threads.reserve(parts);
+        for (; started < parts; ++started) threads.emplace_back(fill, edge(started), edge(started + 1));
+    } catch (const std::exception&) {
+    }
+    fill(0, edge(1));
+    if (started < parts) fill(edge(started), n);
+    for (std::thread& t : threads) t.join();
     float *dc = nullptr, *ds = nullptr;
     const size_t bytes = cs.size() * sizeof(float);
     cudaError_t e = cudaMalloc(&dc, bytes);
