@@ -484,83 +484,81 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
     if (tid < 2 && !(have >> tid & 1)) shared_of(a)[c * 2 + tid].nrec = 0;
 }
 
-// CTA c joins the unit whose first range is c and, with weights, adds those of the parts of shared
-// units that lie in range c. Beside that, before the first launch is done: rows of length 0.
+// CTA (range c, side): if c is the first range of the side's shared unit, joins the unit; with weights,
+// adds those of the range's part of it. Beside that, before the first launch is done: rows of
+// length 0. (One CTA per side rather than one after the other: the chain of latencies is short.)
 __global__ void __launch_bounds__(JOIN_THREADS, 5) attn_paged_join_kernel(const PagedAttnArgs a) {
     __shared__ float s_f[CTAS][GROUP];                       // factor of each record
     __shared__ float red[2 * GROUP][JOIN_THREADS / 32];
     __shared__ __align__(16) float s_sum[JOIN_GROUPS][GROUP * D];
     static_assert(CTAS <= JOIN_THREADS && GROUP * D == JOIN_THREADS, "one record, and one column, a thread");
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x >> 1;
     const int row_floats = GROUP * a.kv.hkv * D;
-    for (int b = tid; b < a.n && c == 0; b += JOIN_THREADS)
+    for (int b = tid; b < a.n && blockIdx.x == 0; b += JOIN_THREADS)
         if (a.lengths[b] != row_length(a, b)) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
-    for (int i = c; i < a.n_layers * a.n; i += CTAS)
+    for (int i = blockIdx.x; i < a.n_layers * a.n; i += gridDim.x)
         if (row_length(a, i % a.n) == 0)
             for (int j = tid * 4; j < row_floats; j += JOIN_THREADS * 4)
                 *reinterpret_cast<float4*>(a.out + (size_t)i * row_floats + j) = make_float4(0.f, 0.f, 0.f, 0.f);
     asm volatile("griddepcontrol.wait;" ::: "memory");       // the split launch is complete and its stores visible
-    for (int side = 0; side < 2; ++side) {
-        const Shared s = shared_of(a)[c * 2 + side];
-        if (s.nrec == 0 || (s.first != c && !a.add_weights)) continue;
-        // record i of the unit: range first + i, slot 0 but in the first range
-        const float* first = a.records + ((size_t)s.first * 2 + s.first_slot) * PARTIAL_FLOATS;
-        const float* others = a.records + (size_t)s.first * 2 * PARTIAL_FLOATS;
-        float M[GROUP] = {-INFINITY, -INFINITY}, L[GROUP] = {0.f, 0.f};
-        float4 st = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
-        if (tid < s.nrec) st = *reinterpret_cast<const float4*>(tid ? others + (size_t)tid * 2 * PARTIAL_FLOATS : first);
-        M[0] = st.x; M[1] = st.y;
+    const Shared s = shared_of(a)[blockIdx.x];
+    if (s.nrec == 0 || (s.first != c && !a.add_weights)) return;
+    // record i of the unit: range first + i, slot 0 but in the first range
+    const float* first = a.records + ((size_t)s.first * 2 + s.first_slot) * PARTIAL_FLOATS;
+    const float* others = a.records + (size_t)s.first * 2 * PARTIAL_FLOATS;
+    float M[GROUP] = {-INFINITY, -INFINITY}, L[GROUP] = {0.f, 0.f};
+    float4 st = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+    if (tid < s.nrec) st = *reinterpret_cast<const float4*>(tid ? others + (size_t)tid * 2 * PARTIAL_FLOATS : first);
+    M[0] = st.x; M[1] = st.y;
+    #pragma unroll
+    for (int k = 0; k < GROUP; ++k) {
         #pragma unroll
-        for (int k = 0; k < GROUP; ++k) {
-            #pragma unroll
-            for (int x = 16; x >= 1; x >>= 1) M[k] = fmaxf(M[k], __shfl_xor_sync(0xffffffffu, M[k], x));
+        for (int x = 16; x >= 1; x >>= 1) M[k] = fmaxf(M[k], __shfl_xor_sync(0xffffffffu, M[k], x));
+    }
+    if (lane < GROUP) red[lane][warp] = lane ? M[1] : M[0];
+    __syncthreads();
+    #pragma unroll
+    for (int k = 0; k < GROUP; ++k)
+        #pragma unroll
+        for (int w = 0; w < JOIN_THREADS / 32; ++w) M[k] = fmaxf(M[k], red[k][w]);
+    if (tid < s.nrec) {
+        const float f0 = exp2_from(st.x, M[0]), f1 = exp2_from(st.y, M[1]);
+        s_f[tid][0] = f0; s_f[tid][1] = f1;
+        L[0] = f0 * st.z; L[1] = f1 * st.w;
+    }
+    #pragma unroll
+    for (int k = 0; k < GROUP; ++k) {
+        #pragma unroll
+        for (int x = 16; x >= 1; x >>= 1) L[k] += __shfl_xor_sync(0xffffffffu, L[k], x);
+    }
+    if (lane < GROUP) red[GROUP + lane][warp] = lane ? L[1] : L[0];
+    __syncthreads();
+    #pragma unroll
+    for (int k = 0; k < GROUP; ++k) {
+        L[k] = 0.f;
+        #pragma unroll
+        for (int w = 0; w < JOIN_THREADS / 32; ++w) L[k] += red[GROUP + k][w];
+    }
+    if (s.first == c) {
+        // four columns a thread, every fourth record a group, then the groups in order
+        const int grp = tid / (GROUP * D / 4), col = tid % (GROUP * D / 4) * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        #pragma unroll 4
+        for (int i = grp; i < s.nrec; i += JOIN_GROUPS) {
+            const float4 x = *reinterpret_cast<const float4*>((i ? others + (size_t)i * 2 * PARTIAL_FLOATS : first) + 4 + col);
+            const float f = s_f[i][col >= D];
+            o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
         }
-        __syncthreads();                                     // s_f, red and s_sum are free
-        if (lane < GROUP) red[lane][warp] = lane ? M[1] : M[0];
+        *reinterpret_cast<float4*>(&s_sum[grp][col]) = o;
         __syncthreads();
+        float sum = 0.f;
         #pragma unroll
-        for (int k = 0; k < GROUP; ++k)
-            #pragma unroll
-            for (int w = 0; w < JOIN_THREADS / 32; ++w) M[k] = fmaxf(M[k], red[k][w]);
-        if (tid < s.nrec) {
-            const float f0 = exp2_from(st.x, M[0]), f1 = exp2_from(st.y, M[1]);
-            s_f[tid][0] = f0; s_f[tid][1] = f1;
-            L[0] = f0 * st.z; L[1] = f1 * st.w;
-        }
-        #pragma unroll
-        for (int k = 0; k < GROUP; ++k) {
-            #pragma unroll
-            for (int x = 16; x >= 1; x >>= 1) L[k] += __shfl_xor_sync(0xffffffffu, L[k], x);
-        }
-        if (lane < GROUP) red[GROUP + lane][warp] = lane ? L[1] : L[0];
-        __syncthreads();
-        #pragma unroll
-        for (int k = 0; k < GROUP; ++k) {
-            L[k] = 0.f;
-            #pragma unroll
-            for (int w = 0; w < JOIN_THREADS / 32; ++w) L[k] += red[GROUP + k][w];
-        }
-        if (s.first == c) {
-            // four columns a thread, every fourth record a group, then the groups in order
-            const int grp = tid / (GROUP * D / 4), col = tid % (GROUP * D / 4) * 4;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            #pragma unroll 4
-            for (int i = grp; i < s.nrec; i += JOIN_GROUPS) {
-                const float4 x = *reinterpret_cast<const float4*>((i ? others + (size_t)i * 2 * PARTIAL_FLOATS : first) + 4 + col);
-                const float f = s_f[i][col / D];
-                o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
-            }
-            *reinterpret_cast<float4*>(&s_sum[grp][col]) = o;
-            __syncthreads();
-            float sum = 0.f;
-            #pragma unroll
-            for (int k = 0; k < JOIN_GROUPS; ++k) sum += s_sum[k][tid];
-            a.out[(size_t)s.unit * GROUP * D + tid] = sum / L[tid / D];
-        }
-        if (a.add_weights) {
-            const int lb = s.unit / a.kv.hkv, b = lb % a.n;
-            add_weights(a, lb / a.n, b, s.unit % a.kv.hkv, row_length(a, b), s.blk0, s.cnt, s.g, M, L, tid, JOIN_THREADS);
-        }
+        for (int k = 0; k < JOIN_GROUPS; ++k) sum += s_sum[k][tid];
+        a.out[(size_t)s.unit * GROUP * D + tid] = sum / (tid < D ? L[0] : L[1]);
+    }
+    if (a.add_weights) {
+        const int lb = s.unit / a.kv.hkv, b = lb % a.n;
+        add_weights(a, lb / a.n, b, s.unit % a.kv.hkv, row_length(a, b), s.blk0, s.cnt, s.g, M, L, tid, JOIN_THREADS);
     }
 }
 
@@ -578,9 +576,9 @@ size_t paged_attn_workspace(int n, int n_layers, int hkv, int max_rows, bool wei
 
 // A launch whose CTAs may start while the launch before it ends; they wait for its end themselves.
 template <class... Params, class... Args>
-static cudaError_t launch_dependent(void (*kernel)(Params...), int threads, size_t smem, cudaStream_t s, const Args&... args) {
+static cudaError_t launch_dependent(void (*kernel)(Params...), int ctas, int threads, size_t smem, cudaStream_t s, const Args&... args) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(CTAS); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
@@ -591,7 +589,7 @@ static cudaError_t launch_dependent(void (*kernel)(Params...), int threads, size
 template <bool WEIGHTS>
 static cudaError_t launch_split(const PagedAttnArgs& a, const CUtensorMap& map, cudaStream_t s) {
     const cudaError_t e = cudaFuncSetAttribute(attn_paged_split_kernel<WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING);
-    return e != cudaSuccess ? e : launch_dependent(attn_paged_split_kernel<WEIGHTS>, THREADS, RING, s, a, map);
+    return e != cudaSuccess ? e : launch_dependent(attn_paged_split_kernel<WEIGHTS>, CTAS, THREADS, RING, s, a, map);
 }
 
 cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* workspace, cudaStream_t s) {
@@ -600,7 +598,7 @@ cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* wor
     a.shared = ws + RECORD_BYTES;
     a.logits = reinterpret_cast<float*>(ws + RECORD_BYTES + SHARED_BYTES);
     const cudaError_t e = a.add_weights ? launch_split<true>(a, map, s) : launch_split<false>(a, map, s);
-    return e != cudaSuccess ? e : launch_dependent(attn_paged_join_kernel, JOIN_THREADS, 0, s, a);
+    return e != cudaSuccess ? e : launch_dependent(attn_paged_join_kernel, CTAS * 2, JOIN_THREADS, 0, s, a);
 }
 
 }  // namespace qattn
