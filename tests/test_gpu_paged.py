@@ -753,3 +753,164 @@ def test_bad_lengths_pages_and_positions_are_reported_and_skipped():
             i = kept[b, 1, 1].long()
             assert torch.equal(c.rows(b, 50)[1, :, 1].view(torch.int16), rows[b][1, :, 1, i].view(torch.int16))
         assert torch.equal(c.kv[spare].view(torch.int16), e.kv[spare].view(torch.int16))
+
+
+# ---- sequences over the cache ----------------------------------------------------------------------
+def test_sequences_follow_the_slot_model():
+    """Prompts, steps, closing and opening through PagedSequences against AttentionModel over slots."""
+    from fpga_qwen_b200.engine import AttentionModel
+    from fpga_qwen_b200.paged import PagedSequences
+    L, steps = 2, 20
+    ctx = make(L, 8, context=1024)
+    qw, kw = H.norms(71, L)
+    H.set_norms(ctx, qw, kw)
+    ref = make(L, 8, context=1024, max_seqs=3)
+    H.set_norms(ref, qw, kw)
+    s = PagedSequences(ctx, n_pages=120, page_rows=16, max_seqs=4, max_rows=700)
+    prompts = {0: 600, 1: 33, 2: 1}
+    models = {}
+    for slot, n in prompts.items():
+        seq = s.open()
+        assert seq == slot
+        q, k, v = H.inputs(100 + slot, L, 0, n)
+        models[slot] = AttentionModel(ref, slot)
+        want, got = models[slot].prefill(q, k, v), s.prefill(seq, q, k, v)
+        # the slot model decodes one-row prompts; both lie within the tolerance of the oracle
+        assert float((want - got).abs().max()) < 2 * H.MAX_ABS
+    for i in range(steps):
+        if i == 10:
+            s.close(1)
+        s.begin_step()
+        q, k, v = (torch.randn(L, 4, h, D, device="cuda") for h in (16, 8, 8))
+        qn, out = torch.empty_like(q), torch.empty_like(q)
+        for layer in range(L):                          # the engine's order: layer by layer
+            one = slice(layer, layer + 1)
+            s.append(q[one], k[one], v[one], layer, q_out=qn[one])
+            s.attend(qn[one], layer, out=out[one])
+        for slot in s.host.live():
+            want = models[slot].step(*(t[:, slot:slot + 1].contiguous() for t in (q, k, v)))
+            assert s.position(slot) == models[slot].position == s.rows(slot)
+            # two FP32 evaluations of the same rows: each within U * (sqrt(128) * |logit| + 2 sqrt(rows)) * 8 < 2e-4 of |v| <= 5
+            assert float((want - out[:, slot:slot + 1]).abs().max()) < 2e-3
+        assert not out[:, 3].any() and (i < 10 or not out[:, 1].any())
+    assert len(s.host.free) == 120 - -(-620 // 16) - -(-21 // 16)
+    ctx.sync()
+    seq = s.open()                                      # a closed sequence's place and pages are used again
+    assert seq == 1
+    q, k, v = H.inputs(200, L, 0, 50)
+    models[1].reset()
+    want, got = models[1].prefill(q, k, v), s.prefill(1, q, k, v)
+    assert float((want - got).abs().max()) < 2 * H.MAX_ABS
+    with pytest.raises(qattn.QAttnError):
+        s.prefill(1, q, k, v)
+    with pytest.raises(qattn.QAttnError):
+        s.prefill(3, q, k, v)
+    with pytest.raises(qattn.QAttnError):
+        s.append(q, k, v)
+    ctx.sync()
+
+
+def test_sequences_keep_a_budget_by_eviction():
+    """A sequence decodes far past its cache: rows stay under the budget, positions go on, and the
+    outputs are those of attention over the kept rows."""
+    from fpga_qwen_b200.paged import PagedSequences
+    L, budget, recent = 2, 64, 16
+    ctx = make(L, 4, context=256)
+    s = PagedSequences(ctx, n_pages=14, page_rows=16, max_seqs=2, max_rows=96, max_position=5000)
+    seq = s.open()
+    g = torch.Generator("cuda").manual_seed(1)
+    q, k, v = (torch.randn(L, 40, h, D, device="cuda", generator=g) for h in (8, 4, 4))
+    s.prefill(seq, q, k, v)
+    keys, values = [], []                               # per step: the cached rows, as FP16
+    for i in range(150):
+        s.begin_step()
+        q, k, v = (torch.randn(L, 2, h, D, device="cuda", generator=g) for h in (8, 4, 4))
+        qn = s.append(q, k, v)
+        out = s.attend(qn)
+        n = s.rows(seq)
+        t = torch.arange(n, device="cuda")
+        ids, at = s.table[seq].long()[t // 16], t % 16
+        rows = s.kv[ids, :, :, :, at].permute(1, 2, 3, 0, 4).double()
+        p = torch.softmax(torch.einsum("lhgd,lhtd->lhgt", qn[:, 0].double().view(L, 4, 2, D), rows[:, 0]) / math.sqrt(D), -1)
+        want = torch.einsum("lhgt,lhtd->lhgd", p, rows[:, 1]).reshape(L, 8, D)
+        # U * (sqrt(128) * 40 + 2 * sqrt(96)) * 8 < 3e-4 of |v| <= 5
+        assert float((out[:, 0].double() - want).abs().max()) < 1.5e-3
+        assert not out[:, 1].any()
+        if n >= 90:
+            held = s.weights[ids, :, :, at].permute(1, 2, 0).cpu().numpy()
+            kept = s.evict(budget, recent)
+            assert s.rows(seq) == budget and s.position(seq) == 41 + i
+            for layer in range(L):
+                for h in range(4):
+                    assert kept[seq, layer, h].tolist() == kept_rows(held[layer, h].tolist(), budget, recent)
+    assert s.position(seq) == 190 and len(s.host.free) == 14 - -(-s.rows(seq) // 16)
+    assert s.lengths.tolist() == [s.rows(seq), 0]
+    with pytest.raises(qattn.QAttnError):
+        s.evict(0)
+    ctx.sync()
+
+
+def test_sequences_captured_steps_stay_valid_and_shapes_are_checked():
+    """One captured step (append and attention of every layer) replayed while sequences grow, close and
+    are evicted gives the same as the calls; wrong shapes are refused."""
+    from fpga_qwen_b200.paged import PagedSequences
+    L, hkv = 2, 2
+
+    def build():
+        ctx = make(L, hkv, context=128)
+        s = PagedSequences(ctx, n_pages=40, page_rows=16, max_seqs=3, max_rows=128, max_position=1000)
+        g = torch.Generator("cuda").manual_seed(9)
+        for n in (50, 17, 1):
+            q, k, v = (torch.randn(L, n, h, D, device="cuda", generator=g) for h in (4, 2, 2))
+            s.prefill(s.open(), q, k, v)
+        return ctx, s
+    results = []
+    for captured in (True, False):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            ctx, s = build()
+            q, k, v = (torch.zeros(L, 3, h, D, device="cuda") for h in (4, 2, 2))
+            qn, out = torch.empty_like(q), torch.empty_like(q)
+
+            def step():
+                s.append(q, k, v, q_out=qn)
+                s.attend(qn, out=out)
+            run = step
+            if captured:
+                stream.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=stream):
+                    step()
+                run = graph.replay
+            seen = []
+            g = torch.Generator("cuda").manual_seed(10)
+            for i in range(40):
+                if i == 15:
+                    s.close(1)
+                if i == 20:
+                    s.evict(32, 8)
+                s.begin_step()
+                for t in (q, k, v):
+                    t.copy_(torch.randn(t.shape, device="cuda", generator=g))
+                run()
+                seen.append(out.clone())
+            stream.synchronize()
+            ctx.sync()
+            results.append(seen)
+            for bad in (lambda: s.attend(qn[:, :2]), lambda: s.attend(qn.half()), lambda: s.append(q, k, v, q_out=qn[:1]),
+                        lambda: s.attend(qn, out=out[:1]), lambda: s.append(q, k[..., :64], v)):
+                with pytest.raises(qattn.QAttnError) as err:
+                    bad()
+                assert err.value.status == qattn.QA_ERR_INVALID
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+    ctx = make(L, hkv, context=128)
+    one = PagedSequences(ctx, n_pages=4, max_seqs=1, max_rows=32, step_layers=1)
+    one.open()
+    one.begin_step()
+    q, k, v = (torch.randn(L, 1, h, D, device="cuda") for h in (4, 2, 2))
+    qn = one.append(q, k, v)
+    one.attend(qn[1:], 1)
+    with pytest.raises(qattn.QAttnError):
+        one.attend(qn)                                  # its workspace holds one layer
+    ctx.sync()
