@@ -134,15 +134,20 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const PagedEv
             if (lane >= o) incl += x;
         }
         const int at = __ffs(__ballot_sync(0xffffffffu, incl >= need)) - 1;
-        int before = incl - sum, bin = BINS - 1 - 8 * lane;
+        int before = incl - sum, bin = BINS - 1 - 8 * lane, in_bin = v[0];
         bool found = false;
         #pragma unroll
         for (int i = 0; i < 7; ++i) {
             found = found || before + v[i] >= need;
-            if (!found) { before += v[i]; --bin; }
+            if (!found) { before += v[i]; --bin; in_bin = v[i + 1]; }
         }
         prefix |= (unsigned)__shfl_sync(0xffffffffu, bin, at) << shift;
         need -= __shfl_sync(0xffffffffu, before, at);
+        if (need == __shfl_sync(0xffffffffu, in_bin, at) && prefix) {
+            --prefix;                                        // the whole bin stays: no need to look inside
+            need = 0;
+            break;
+        }
     }
     // ---- ascending pass: each warp takes a run of the slice's rows; first it counts ----
     const int run = ((rows + SEL_WARPS - 1) / SEL_WARPS + 31) & ~31;
