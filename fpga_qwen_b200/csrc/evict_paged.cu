@@ -33,7 +33,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32;
-constexpr int BINS = 256, BATCH = 8;
+constexpr int BINS = 256, BATCH = 4;
 constexpr int SLICE_ROWS = 4096;                   // of a cluster's CTA, where there are SMs for it
 constexpr int MAX_SLICE = 49152;                   // 192 KB of shared memory
 constexpr int TABLE_INTS = 1024;                   // page ids of the destination kept in shared memory
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const PagedEv
     for (int pass = 0; pass < 4 && wanted; ++pass) {
         const int shift = 24 - 8 * pass;
         const unsigned known = pass ? ~0u << (shift + 8) : 0u;
-        #pragma unroll 4
+        #pragma unroll 2
         for (int i = tid; i < compete; i += SEL_THREADS) {
             const unsigned k = evict_key(s_w[i]);
             if (((k ^ prefix) & known) == 0) atomicAdd(&hist[pass][(k >> shift) & (BINS - 1)], 1);
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const PagedEv
             cluster.sync();
             if (tid < BINS) {
                 int sum = 0;
-                #pragma unroll 4
+                #pragma unroll 2
                 for (int r = 0; r < ranks; ++r) sum += cluster.map_shared_rank(hist[pass], r)[tid];
                 bins[pass & 1][tid] = sum;
             }
@@ -203,20 +203,24 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const PagedEv
     if (ranks > 1) cluster.sync();                           // until the others have read this CTA's memory
 }
 
-constexpr int MOVE_THREADS = 256, UNROLL = 4;
-constexpr int MOVE_ROWS = MOVE_THREADS / 16;       // rows per load: 16 threads of 16 bytes each
+constexpr int MOVE_THREADS = 256;
+constexpr int ROW_THREADS = 8, CHUNKS = 16 / ROW_THREADS;    // threads of a row; 16-byte chunks of a thread
+constexpr int PER_THREAD = 2;                                // rows of a thread and tile
+constexpr int MOVE_ROWS = MOVE_THREADS / ROW_THREADS, TILE = MOVE_ROWS * PER_THREAD;
 
-// Cluster (unit, K|V): moves the kept rows, tile after tile of UNROLL * MOVE_ROWS rows per CTA. Three
-// tiles are under way: one being stored, the next one's rows and the one after's indices and
-// pages being loaded. A tile's rows may be loaded before the tile before it is stored, since its
-// sources lie above those destinations.
+// Cluster (unit, K|V): moves the kept rows, tile after tile of TILE rows per CTA. Three tiles are
+// under way: one being stored, the next one's rows and the one after's indices and pages being
+// loaded. A tile's rows may be loaded before the tile before it is stored, since its sources lie
+// above those destinations. Eight threads take a row, two 16-byte chunks each: with
+// sixteen, one chunk each, half of the issue slots went to indices and addresses, which cost a few
+// per cent.
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const PagedEvictArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
-    const int unit = blockIdx.x / ranks, kv = blockIdx.y, tile = UNROLL * MOVE_ROWS * ranks;
+    const int unit = blockIdx.x / ranks, kv = blockIdx.y, tile = TILE * ranks;
     const int h = unit % a.kv.hkv, layer = (unit / a.kv.hkv) % a.kv.layers, b = unit / (a.kv.hkv * a.kv.layers);
     const int mask = (1 << a.kv.shift) - 1;
-    const int chunk = threadIdx.x & 15, r = rank * (UNROLL * MOVE_ROWS) + (threadIdx.x >> 4);
+    const int chunk = threadIdx.x % ROW_THREADS, r = rank * TILE + threadIdx.x / ROW_THREADS;
     const int* kept = a.kept + (size_t)unit * a.keep;
     const int* src = a.src_table + (size_t)b * a.src_cols;
     const int* dst = a.dst_table + (size_t)b * a.dst_cols;
@@ -229,29 +233,33 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const PagedEvi
         }
         a.new_lengths[b] = lo;
     }
-    int from[UNROLL], page[UNROLL], to[UNROLL];    // of the tile ahead: old row, its page, the new row's page (-1: no move)
+    int from[PER_THREAD], page[PER_THREAD], to[PER_THREAD];  // of the tile ahead: old row, its page, the new row's page (-1: no move)
     auto load_index = [&](int j0) {
         #pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
+        for (int i = 0; i < PER_THREAD; ++i) {
             const int j = j0 + i * MOVE_ROWS + r;
             from[i] = j < a.keep ? __ldg(kept + j) : -1;
         }
     };
     auto load_pages = [&](int j0) {
         #pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
+        for (int i = 0; i < PER_THREAD; ++i) {
             const int j = j0 + i * MOVE_ROWS + r;
             page[i] = from[i] < 0 ? -1 : __ldg(src + (from[i] >> a.kv.shift));
             to[i] = from[i] < 0 ? -1 : __ldg(dst + (j >> a.kv.shift));
         }
     };
-    uint4 v[UNROLL], next[UNROLL];
-    int dest[UNROLL], next_dest[UNROLL];           // page to store to, or -1
-    auto load_rows = [&](uint4 (&x)[UNROLL], int (&d)[UNROLL]) {
+    uint4 v[PER_THREAD][CHUNKS], next[PER_THREAD][CHUNKS];
+    int dest[PER_THREAD], next_dest[PER_THREAD];   // page to store to, or -1
+    auto load_rows = [&](uint4 (&x)[PER_THREAD][CHUNKS], int (&d)[PER_THREAD]) {
         #pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
+        for (int i = 0; i < PER_THREAD; ++i) {
             d[i] = a.kv.has(page[i]) && a.kv.has(to[i]) ? to[i] : -1;      // (bad pages are recorded by the selection)
-            if (d[i] >= 0) x[i] = reinterpret_cast<const uint4*>(a.kv.row(page[i], layer, kv, h, from[i] & mask))[chunk];
+            if (d[i] >= 0) {
+                const uint4* p = reinterpret_cast<const uint4*>(a.kv.row(page[i], layer, kv, h, from[i] & mask)) + chunk;
+                #pragma unroll
+                for (int k = 0; k < CHUNKS; ++k) x[i][k] = p[k * ROW_THREADS];
+            }
         }
     };
     load_index(0);
@@ -264,10 +272,15 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const PagedEvi
         load_index(min(j0 + 2 * tile, a.keep));
         if (ranks > 1) cluster.sync(); else __syncthreads();   // every thread has its rows of this tile
         #pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
+        for (int i = 0; i < PER_THREAD; ++i) {
             const int j = j0 + i * MOVE_ROWS + r;
-            if (dest[i] >= 0) reinterpret_cast<uint4*>(a.kv.row(dest[i], layer, kv, h, j & mask))[chunk] = v[i];
-            v[i] = next[i];
+            if (dest[i] >= 0) {
+                uint4* p = reinterpret_cast<uint4*>(a.kv.row(dest[i], layer, kv, h, j & mask)) + chunk;
+                #pragma unroll
+                for (int k = 0; k < CHUNKS; ++k) p[k * ROW_THREADS] = v[i][k];
+            }
+            #pragma unroll
+            for (int k = 0; k < CHUNKS; ++k) v[i][k] = next[i][k];
             dest[i] = next_dest[i];
         }
         load_pages(j0 + 2 * tile);
@@ -310,7 +323,7 @@ cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t s) {
     // move: clusters that fill the GPU (4 CTAs per SM) where the units alone do not and there are rows
     // for every CTA
     ranks = 1;
-    while (ranks < 16 && units * 2 * ranks * 2 <= 4 * NUM_SMS_B200 && ranks * UNROLL * MOVE_ROWS < a.keep) ranks *= 2;
+    while (ranks < 16 && units * 2 * ranks * 2 <= 4 * NUM_SMS_B200 && ranks * TILE < a.keep) ranks *= 2;
     return launch(evict_move_kernel, dim3(units, 2), MOVE_THREADS, 0, ranks, true, a, s);
 }
 
