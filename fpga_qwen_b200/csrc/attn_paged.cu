@@ -196,7 +196,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
         prefetch_tmap(&map);
     }
     if (tid < WARPS * 2) parts[tid >> 1][tid & 1].unit = -1;
-    asm volatile("griddepcontrol.wait;" ::: "memory");       // what ran before is complete
+    // What ran before is complete. (No read-only loads below: they may move across this, and what it
+    // waits for may write the queries, tables and lengths.)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const PagedSplit sp = scan_lengths(a, start, warp_sum);   // its barriers publish the above too
     if (sp.total == 0 || c >= sp.ctas) {
@@ -220,13 +222,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
         float4 q_raw[2];
         auto load_q = [&](const PagedUnit& w) {
             const float* row = a.q + ((((size_t)w.l * a.n + w.b) * hkv + w.kh) * GROUP) * D + lane * 8;
-            q_raw[0] = __ldg(reinterpret_cast<const float4*>(row));
-            q_raw[1] = __ldg(reinterpret_cast<const float4*>(row) + 1);
+            q_raw[0] = reinterpret_cast<const float4*>(row)[0];
+            q_raw[1] = reinterpret_cast<const float4*>(row)[1];
         };
         int page_next = -1, place_next = 0;                  // next batch: page id, first row within the page's K rows of the head
         auto look_up = [&](const PagedUnit& w, long long g) {
             const int t0 = (int)(g - w.off) * BLK;
-            page_next = __ldg(a.table + (size_t)w.b * a.cols + (t0 >> a.kv.shift));
+            page_next = a.table[(size_t)w.b * a.cols + (t0 >> a.kv.shift)];
             place_next = (((a.layer0 + w.l) * 2 * hkv + w.kh) << a.kv.shift) + (t0 & mask);
         };
         // row of the block's K in the pool's matrix of planes ((page, layer), K|V, head); -1: no such page

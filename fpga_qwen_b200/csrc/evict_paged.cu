@@ -211,7 +211,7 @@ constexpr int MOVE_ROWS = MOVE_THREADS / ROW_THREADS, TILE = MOVE_ROWS * PER_THR
 // Cluster (unit, K|V): moves the kept rows, tile after tile of TILE rows per CTA. Three tiles are
 // under way: one being stored, the next one's rows and the one after's indices and pages being
 // loaded. A tile's rows may be loaded before the tile before it is stored, since its sources lie
-// above those destinations. Eight threads take a row, two 16-byte chunks each: with
+// above those destinations. Rows that are in place already are not touched. Eight threads take a row, two 16-byte chunks each: with
 // sixteen, one chunk each, half of the issue slots went to indices and addresses, which cost a few
 // per cent.
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const PagedEvictArgs a) {
@@ -224,7 +224,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const PagedEvi
     const int* kept = a.kept + (size_t)unit * a.keep;
     const int* src = a.src_table + (size_t)b * a.src_cols;
     const int* dst = a.dst_table + (size_t)b * a.dst_cols;
-    asm volatile("griddepcontrol.wait;" ::: "memory");       // the selection is complete
+    // The selection is complete. (No read-only loads of what it writes: they may move across this.)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (layer == 0 && h == 0 && kv == 0 && rank == 0 && threadIdx.x == 0) {
         int lo = 0, hi = a.keep;                   // kept rows: the first -1
         while (lo < hi) {
@@ -238,15 +239,16 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const PagedEvi
         #pragma unroll
         for (int i = 0; i < PER_THREAD; ++i) {
             const int j = j0 + i * MOVE_ROWS + r;
-            from[i] = j < a.keep ? __ldg(kept + j) : -1;
+            from[i] = j < a.keep ? kept[j] : -1;
         }
     };
     auto load_pages = [&](int j0) {
         #pragma unroll
         for (int i = 0; i < PER_THREAD; ++i) {
             const int j = j0 + i * MOVE_ROWS + r;
-            page[i] = from[i] < 0 ? -1 : __ldg(src + (from[i] >> a.kv.shift));
-            to[i] = from[i] < 0 ? -1 : __ldg(dst + (j >> a.kv.shift));
+            page[i] = from[i] < 0 ? -1 : src[from[i] >> a.kv.shift];
+            to[i] = from[i] < 0 ? -1 : dst[j >> a.kv.shift];
+            if (page[i] == to[i] && ((from[i] ^ j) & mask) == 0) to[i] = -1;   // in place already
         }
     };
     uint4 v[PER_THREAD][CHUNKS], next[PER_THREAD][CHUNKS];

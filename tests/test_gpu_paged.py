@@ -363,6 +363,42 @@ def test_offsets_past_32_bits():
     ctx.sync()
 
 
+def test_weights_gathered_by_two_streams_into_one_pool():
+    """Calls that accumulate into the same pages from two streams, each with its own workspace: every
+    call's weights arrive (their additions come in any order)."""
+    ctx = make(1, 4)
+    c = Cache([900, 400], 1, 4, page=32, seed=16)
+    q = [c.query() for _ in range(2)]
+    before = [c.weights(b).double().clone() for b in range(2)]
+    size = ctx.paged_workspace(2, 1, c.cols * c.page, True)
+    lens = i32(c.lengths)
+    spaces = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    outs = [torch.empty_like(x) for x in q]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, x, out, ws in zip(streams, q, outs, spaces):
+            ctx.set_stream(s.cuda_stream)
+            ctx.paged_attn(c.pages, c.table.data_ptr(), c.cols, lens.data_ptr(), 2, 0, 1, x.data_ptr(), out.data_ptr(), True,
+                           ws.data_ptr(), size)
+    torch.cuda.synchronize()
+    for b in range(2):
+        total, limit = before[b].clone(), torch.zeros_like(before[b])
+        for x in q:
+            _, _, probs = reference(c, x)
+            total += 5 * probs[b][0]
+            limit += 5 * probs[b][1]
+        assert bool(((c.weights(b).double() - total).abs() <= limit + 20 * U * total).all())
+
+
+def test_lengths_up_to_the_tables_capacity_and_pages_at_the_pools_ends():
+    ctx = make(2, 2)
+    for page in (16, 512):
+        c = Cache([3 * page, 3 * page - 1, 1], 2, 2, page=page, seed=17, extra_cols=0, spare=0)
+        assert sorted(c.table[c.table >= 0].tolist()) == list(range(c.n_pages))
+        check_attend(ctx, c, c.query(), add=True)
+
+
 # ---- append --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("hkv,page,n", [(8, 16, 1), (8, 16, 5), (4, 32, 7), (2, 64, 33), (1, 512, 130), (8, 128, 40)])
 def test_append_tokens_bit_exact_with_the_oracle(hkv, page, n):
@@ -507,6 +543,50 @@ def test_evict_into_other_pages(page, keep, recent):
     used = set(c.table.flatten().tolist())
     free = [p for p in range(c.n_pages) if p not in used][:4 * cols]
     check_evict(ctx, c, keep, recent, dst=i32(free).view(4, cols).contiguous())
+
+
+@pytest.mark.parametrize("rows,hkv,layers,page,keep,recent", [
+    (5000, 8, 1, 16, 3000, 100), (40000, 1, 1, 64, 20001, 0), (524288, 1, 1, 512, 300000, 4096), (70000, 2, 1, 128, 1, 1),
+    (9000, 8, 3, 32, 8999, 17), (4097, 4, 28, 64, 100, 0)])
+def test_evict_long_units_over_several_slices(rows, hkv, layers, page, keep, recent):
+    """Units whose rows are spread over a cluster (more than 4096), against a sort."""
+    ctx = make(layers, hkv)
+    g = torch.Generator("cuda").manual_seed(rows)
+    cols = -(-rows // page)
+    table = torch.randperm(cols, device="cuda", generator=g).to(torch.int32)[None].contiguous()
+    kv = torch.randint(-30000, 30000, (cols, layers, 2, hkv, page, D), dtype=torch.int16, device="cuda", generator=g)
+    w = (torch.rand(cols, layers, hkv, page, device="cuda", generator=g) * 50).floor() / 50     # many ties
+    t = torch.arange(rows, device="cuda")
+    ids, at = table[0].long()[t // page], t % page
+    flat_w = w[ids, :, :, at].permute(1, 2, 0)                                                   # [layers][hkv][rows]
+    rank = flat_w.clone()
+    rank[..., rows - recent:] = 2.0
+    want = torch.sort(torch.sort(rank, dim=-1, descending=True, stable=True).indices[..., :keep], dim=-1).values
+    old = kv.clone()
+    lens, new = i32([rows]), i32([0])
+    kept = torch.empty(1, layers, hkv, keep, dtype=torch.int32, device="cuda")
+    ctx.paged_evict(qattn.Pages(kv.data_ptr(), w.data_ptr(), cols, page), table.data_ptr(), cols, table.data_ptr(), cols,
+                    lens.data_ptr(), new.data_ptr(), 1, keep, recent, kept.data_ptr())
+    ctx.sync()
+    assert new.tolist() == [keep] and torch.equal(kept[0].long(), want)
+    got_w = w[ids[:keep], :, :, at[:keep]].permute(1, 2, 0)
+    assert torch.equal(got_w, torch.gather(flat_w, 2, want))
+    for layer in range(layers):
+        for h in range(hkv):
+            i = want[layer, h]
+            assert torch.equal(kv[ids[:keep], layer, :, h, at[:keep]], old[ids[i], layer, :, h, at[i]])
+    assert torch.equal(kv[ids[keep:], :, :, :, at[keep:]], old[ids[keep:], :, :, :, at[keep:]])
+
+
+def test_evict_refuses_tables_beyond_its_rows():
+    ctx = make(1, 8)
+    c = Cache([40], 1, 8, seed=33)
+    lens, new = i32([40]), i32([0])
+    kept = torch.empty(8 * 20, dtype=torch.int32, device="cuda")
+    with pytest.raises(qattn.QAttnError) as err:
+        ctx.paged_evict(c.pages, c.table.data_ptr(), (1 << 19) // 16 + 1, c.table.data_ptr(), c.cols, lens.data_ptr(),
+                        new.data_ptr(), 1, 20, 0, kept.data_ptr())
+    assert err.value.status == qattn.QA_ERR_INVALID
 
 
 def test_evict_ties_zeros_infinities_and_nan():
