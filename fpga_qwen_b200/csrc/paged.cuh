@@ -102,6 +102,19 @@ QA_HD void paged_next_unit(const int* start, int n, int hkv, PagedUnit& u) {
     }
 }
 
+// Short units: range c is unit c (of n_layers * n * hkv) whole, and its blocks begin at c * most,
+// where `most` is the blocks that a table row can hold. `nblk` is filled by the caller.
+QA_HD PagedUnit paged_unit_alone(int c, int n, int hkv, int most) {
+    PagedUnit u;
+    const int lb = c / hkv;
+    u.kh = c - lb * hkv;
+    u.l = lb / n;
+    u.b = lb - u.l * n;
+    u.nblk = 0;
+    u.off = (long long)c * most;
+    return u;
+}
+
 // ---- eviction order -------------------------------------------------------------------------------
 // Larger weight <=> larger key; -0 equals 0; NaN is the lowest.
 QA_HD uint32_t evict_key(float w) {

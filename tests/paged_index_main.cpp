@@ -123,6 +123,22 @@ int main() {
                         walk(valid, cols, shift, layers, hkv, 148, 8, 8);
                         walk(valid, cols, shift, layers, hkv, pick(1, 600), pick(1, 16), pick(1, 16));
                     }
+    // short units: every unit once, its logits in a place of their own inside the workspace
+    for (int n : {1, 3, 18, 148})
+        for (int layers : {1, 2, 28})
+            for (int hkv : {1, 2, 4, 8})
+                for (int most : {1, 7, 32}) {
+                    const int units = n * layers * hkv;
+                    std::vector<int> hit(units, 0);
+                    for (int c = 0; c < units; ++c) {
+                        const PagedUnit u = paged_unit_alone(c, n, hkv, most);
+                        CHECK(u.l >= 0 && u.l < layers && u.b >= 0 && u.b < n && u.kh >= 0 && u.kh < hkv);
+                        CHECK((u.l * n + u.b) * hkv + u.kh == c && u.off == (long long)c * most);
+                        CHECK(u.off + most <= (long long)n * layers * hkv * most);
+                        ++hit[(u.l * n + u.b) * hkv + u.kh];
+                    }
+                    for (int h : hit) CHECK(h == 1);
+                }
     // places: every combination of bad and good length, sequence, position and page id
     for (int shift = 4; shift <= 9; ++shift) {
         const int cols = 3, n_seqs = 4, n_pages = 7;

@@ -399,6 +399,28 @@ def test_lengths_up_to_the_tables_capacity_and_pages_at_the_pools_ends():
         check_attend(ctx, c, c.query(), add=True)
 
 
+@pytest.mark.parametrize("layers,hkv,n,cols_rows", [(1, 8, 18, 512), (1, 1, 148, 512), (1, 1, 149, 512), (28, 1, 5, 256), (2, 8, 3, 513)])
+def test_short_units_around_the_rule_for_one_cta_each(layers, hkv, n, cols_rows):
+    """Calls on either side of the rule (units and rows that a table can hold), ragged with empty rows."""
+    ctx = make(layers, hkv)
+    r = np.random.default_rng(n)
+    lengths = [int(x) for x in r.integers(0, cols_rows + 1, n)]
+    lengths[0], lengths[-1] = cols_rows, 0 if n > 1 else cols_rows
+    c = Cache(lengths, layers, hkv, page=16, seed=n, extra_cols=0)
+    check_attend(ctx, c, c.query(), add=True)
+    check_attend(ctx, c, c.query())
+    # lengths outside the table: zeros for that row, reported
+    q = c.query()
+    want, tol, _ = reference(c, q)
+    bad = i32(lengths)
+    bad[0] = c.cols * 16 + 1
+    out = attend(ctx, c, q, lengths=bad)
+    with pytest.raises(qattn.QAttnError) as err:
+        ctx.sync()
+    assert "code 61" in str(err.value) and not out[:, 0].any()
+    assert bool(((out.double() - want).abs() <= tol)[:, 1:].all())
+
+
 # ---- append --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("hkv,page,n", [(8, 16, 1), (8, 16, 5), (4, 32, 7), (2, 64, 33), (1, 512, 130), (8, 128, 40)])
 def test_append_tokens_bit_exact_with_the_oracle(hkv, page, n):
