@@ -43,13 +43,16 @@
 // CTA or, for units shared between CTAs, in the joining launch, each CTA those of its own range.
 // Each (row, KV head) weight gets one FP32 addition.
 //
-// Short units need none of that: where a table row holds at most ALONE_ROWS rows and there are no
-// more units than SMs, every unit is one CTA's, without the scan of the lengths and without the
-// second launch (8 units of 256 rows 8.4 -> 5.7 us, of 512 rows 8.4 -> 7.7 us, 144 units of 512 rows
-// 13.7 -> 8.4 us; longer tables lose with few units or with ragged lengths).
+// Calls of few units that are not long need none of that: every unit has a CTA, or a cluster of two or
+// four, of its own, without the scan of the lengths, and a cluster's CTAs join their parts over
+// distributed shared memory, without the second launch (paged_ctas_alone says when: 8 units of 256
+// rows 8.6 -> 5.9 us, of 1024 rows 9.0 -> 8.0 us, 32 units of 2048 rows 13.7 -> 10.6 us, 144 units
+// of 512 rows 13.7 -> 8.4 us).
 //
 // Every wait is bounded: on expiry the CTA records an error code, consumes no further block, and
 // drains its copies before it exits.
+#include <cooperative_groups.h>
+
 #include "qattn_common.cuh"
 #include "sm100.cuh"
 
@@ -57,6 +60,7 @@ namespace qattn {
 namespace {
 
 using namespace sm100;
+namespace cg = cooperative_groups;
 
 constexpr int WARPS = 8, THREADS = WARPS * 32;
 constexpr int BLK = PAGED_BLK;
@@ -67,7 +71,6 @@ constexpr int RING = WARPS * STAGES * STAGE;
 constexpr int CTAS = NUM_SMS_B200;            // ranges
 constexpr int MIN_BLOCKS = WARPS;             // blocks per range, at least
 constexpr int JOIN_THREADS = 256, JOIN_GROUPS = JOIN_THREADS / (GROUP * D / 4);
-constexpr int ALONE_ROWS = 512;
 constexpr int WAIT_CODE = 43;                 // error code of an expired wait
 
 // A part of a unit that its worker does not finish alone.
@@ -82,6 +85,12 @@ struct __align__(16) Shared {
     int nrec, first, first_slot, unit;        // records of the unit (0: no such part), their first range and its slot
     int blk0, cnt;
     long long g;                              // its first block in the call
+};
+// A CTA's part of its cluster's unit.
+struct Joint {
+    int cnt;                                  // blocks, 0: none
+    float m[GROUP], l[GROUP];
+    float o[GROUP * D];
 };
 __device__ __forceinline__ Shared* shared_of(const PagedAttnArgs& a) { return static_cast<Shared*>(a.shared); }
 
@@ -191,12 +200,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
     __shared__ int warp_sum[WARPS];
     __shared__ Part parts[WARPS][2];                         // [0]: of the warp's first unit, [1]: of its last
     __shared__ __align__(16) float s_part[WARPS][2][GROUP * D];
+    __shared__ Joint joint;
     __shared__ int abort_flag, never_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
     const int g8 = lane >> 2, j4 = lane & 3, head = j4 & 1;  // tile row or column, and the column pair's head
     const int hkv = a.kv.hkv;
     if (tid == 0) {
-        abort_flag = 0; never_abort = 0;
+        abort_flag = 0; never_abort = 0; joint.cnt = 0;
         for (int i = 0; i < WARPS * STAGES; ++i) mbar_init(&full[0][0] + i, 1);
         fence_mbar_init();
         prefetch_tmap(&map);
@@ -211,16 +221,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
     long long c_begin;
     int c_blocks;                                            // at most 2^28 (64 layers, 8 heads, 2^30 rows over 148 ranges)
     if (a.alone) {
-        only = paged_unit_alone(c, a.n, hkv, ((a.cols << a.kv.shift) + BLK - 1) / BLK);
+        const int i = c / a.alone, rank = c - i * a.alone;   // the CTA's unit, and its place in the cluster
+        only = paged_unit_alone(i, a.n, hkv, ((a.cols << a.kv.shift) + BLK - 1) / BLK);
         const int given = a.lengths[only.b], len = paged_length(given, a.cols, a.kv.shift);
         if (given != len && tid == 0) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
         only.nblk = (len + BLK - 1) / BLK;
-        if (len == 0) {
-            a.out[(size_t)c * GROUP * D + tid] = 0.f;
+        if (len == 0) {                                      // (for the whole cluster)
+            if (rank == 0) a.out[(size_t)i * GROUP * D + tid] = 0.f;
             return;
         }
-        c_begin = only.off;
-        c_blocks = only.nblk;
+        const int from = only.nblk * rank / a.alone;
+        c_begin = only.off + from;
+        c_blocks = only.nblk * (rank + 1) / a.alone - from;
         __syncthreads();                                     // the barriers and parts above are ready
     } else {
         sp = scan_lengths(a, start, warp_sum);               // (its barriers cover them too)
@@ -491,6 +503,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
                 const int lb = unit / hkv, row_l = lb / a.n, row_b = lb - row_l * a.n, row_kh = unit - lb * hkv;
                 add_weights(a, row_l, row_b, row_kh, row_length(a, row_b), 0, cnt, g, M, L, tid, THREADS);
             }
+        } else if (a.alone) {
+            joint.o[tid] = o;
+            if (tid < GROUP) { joint.m[tid] = tid ? M[1] : M[0]; joint.l[tid] = tid ? L[1] : L[0]; }
+            if (tid == 0) joint.cnt = cnt;
         } else {
             const int slot = g != c_begin;
             float* rec = a.records + ((size_t)c * 2 + slot) * PARTIAL_FLOATS;
@@ -508,7 +524,50 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
             have |= 1u << slot;
         }
     }
-    if (!a.alone && tid < 2 && !(have >> tid & 1)) shared_of(a)[c * 2 + tid].nrec = 0;
+    if (!a.alone) {
+        if (tid < 2 && !(have >> tid & 1)) shared_of(a)[c * 2 + tid].nrec = 0;
+        return;
+    }
+    if (a.alone == 1) return;
+    // ---- join the cluster's parts (none where one CTA held the whole unit) ----
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    int cnts[4], total = 0;
+    float M[GROUP] = {-INFINITY, -INFINITY}, L[GROUP] = {0.f, 0.f}, f[4][GROUP];
+    #pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        cnts[r] = 0;
+        f[r][0] = f[r][1] = -INFINITY;
+        if (r >= a.alone) continue;
+        const Joint* x = cluster.map_shared_rank(&joint, r);
+        cnts[r] = x->cnt;
+        f[r][0] = x->m[0]; f[r][1] = x->m[1];
+        total += cnts[r];
+    }
+    if (total == only.nblk) {
+        #pragma unroll
+        for (int r = 0; r < 4; ++r)
+            #pragma unroll
+            for (int k = 0; k < GROUP; ++k)
+                if (cnts[r]) M[k] = fmaxf(M[k], f[r][k]);
+        float sum = 0.f;
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (!cnts[r]) continue;
+            const Joint* x = cluster.map_shared_rank(&joint, r);
+            #pragma unroll
+            for (int k = 0; k < GROUP; ++k) {
+                f[r][k] = exp2_from(f[r][k], M[k]);
+                L[k] += f[r][k] * x->l[k];
+            }
+            sum += (tid < D ? f[r][0] : f[r][1]) * x->o[tid];
+        }
+        const int i = c / a.alone;
+        if (c - i * a.alone == 0) a.out[(size_t)i * GROUP * D + tid] = sum / (tid < D ? L[0] : L[1]);
+        if (WEIGHTS && c_blocks)
+            add_weights(a, only.l, only.b, only.kh, row_length(a, only.b), (int)(c_begin - only.off), c_blocks, c_begin, M, L, tid, THREADS);
+    }
+    cluster.sync();                                          // until the others have read this CTA's memory
 }
 
 // CTA (range c, side): if c is the first range of the side's shared unit, joins the unit; with weights,
@@ -603,20 +662,23 @@ size_t paged_attn_workspace(int n, int n_layers, int hkv, int max_rows, bool wei
 
 // A launch whose CTAs may start while the launch before it ends; they wait for its end themselves.
 template <class... Params, class... Args>
-static cudaError_t launch_dependent(void (*kernel)(Params...), int ctas, int threads, size_t smem, cudaStream_t s, const Args&... args) {
+static cudaError_t launch_dependent(void (*kernel)(Params...), int ctas, int cluster, int threads, size_t smem, cudaStream_t s,
+                                    const Args&... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr; cfg.numAttrs = 1;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <bool WEIGHTS>
 static cudaError_t launch_split(const PagedAttnArgs& a, const CUtensorMap& map, int ctas, cudaStream_t s) {
     const cudaError_t e = cudaFuncSetAttribute(attn_paged_split_kernel<WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING);
-    return e != cudaSuccess ? e : launch_dependent(attn_paged_split_kernel<WEIGHTS>, ctas, THREADS, RING, s, a, map);
+    return e != cudaSuccess ? e : launch_dependent(attn_paged_split_kernel<WEIGHTS>, ctas, a.alone > 1 ? a.alone : 1, THREADS, RING, s, a, map);
 }
 
 cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* workspace, cudaStream_t s) {
@@ -625,10 +687,10 @@ cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* wor
     a.shared = ws + RECORD_BYTES;
     a.logits = reinterpret_cast<float*>(ws + RECORD_BYTES + SHARED_BYTES);
     const long long units = (long long)a.n * a.n_layers * a.kv.hkv;
-    a.alone = units <= CTAS && a.cols << a.kv.shift <= ALONE_ROWS;
-    const int ctas = a.alone ? (int)units : CTAS;
+    a.alone = paged_ctas_alone(units, ((a.cols << a.kv.shift) + BLK - 1) / BLK, CTAS, WARPS);
+    const int ctas = a.alone ? (int)units * a.alone : CTAS;
     const cudaError_t e = a.add_weights ? launch_split<true>(a, map, ctas, s) : launch_split<false>(a, map, ctas, s);
-    return e != cudaSuccess || a.alone ? e : launch_dependent(attn_paged_join_kernel, CTAS * 2, JOIN_THREADS, 0, s, a);
+    return e != cudaSuccess || a.alone ? e : launch_dependent(attn_paged_join_kernel, CTAS * 2, 1, JOIN_THREADS, 0, s, a);
 }
 
 }  // namespace qattn

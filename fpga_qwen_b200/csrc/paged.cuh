@@ -102,17 +102,35 @@ QA_HD void paged_next_unit(const int* start, int n, int hkv, PagedUnit& u) {
     }
 }
 
-// Short units: range c is unit c (of n_layers * n * hkv) whole, and its blocks begin at c * most,
-// where `most` is the blocks that a table row can hold. `nblk` is filled by the caller.
-QA_HD PagedUnit paged_unit_alone(int c, int n, int hkv, int most) {
+// Calls of few units: unit i (of n_layers * n * hkv) has CTAs of its own, and its blocks begin at
+// i * most, where `most` is the blocks that a table row can hold. `nblk` is filled by the caller.
+QA_HD PagedUnit paged_unit_alone(int i, int n, int hkv, int most) {
     PagedUnit u;
-    const int lb = c / hkv;
-    u.kh = c - lb * hkv;
+    const int lb = i / hkv;
+    u.kh = i - lb * hkv;
     u.l = lb / n;
     u.b = lb - u.l * n;
     u.nblk = 0;
-    u.off = (long long)c * most;
+    u.off = (long long)i * most;
     return u;
+}
+// CTAs of each unit in such a call (1, 2 or 4; of `warps` warps), or 0: the even split. By estimated
+// times in units of 0.095 us, measured over 8 to 144 units of 1 to 8192 rows: a launch of its own
+// CTAs 44, a cluster's join 18, a block of every warp 10; the even split with its second launch 92,
+// and 13 for each block that its warps have past the first. `most` is the longest row that the
+// table can hold, so a warp gets at most four blocks (ragged lengths leave CTAs idle), and clusters
+// of four take at most 128 SMs (GPCs do not hold a multiple of four).
+QA_HD int paged_ctas_alone(long long units, int most, int max_ctas, int warps) {
+    if (units > max_ctas) return 0;
+    const long long x = units * most * 10 / ((long long)max_ctas * warps);      // blocks per warp, in tenths
+    long long best = 92 + (x > 9 ? (x - 9) * 13 / 10 : 0);
+    int ctas = 0;
+    for (int k = 1; k <= 4; k *= 2) {
+        if (units * k > (k == 4 ? max_ctas - 20 : max_ctas) || most > k * warps * 4) continue;
+        const long long cost = 44 + (k > 1 ? 18 : 0) + (long long)most * 10 / (k * warps);
+        if (cost < best) { best = cost; ctas = k; }
+    }
+    return ctas;
 }
 
 // ---- eviction order -------------------------------------------------------------------------------

@@ -230,7 +230,7 @@ struct PagedAttnArgs {
     PagedKV kv;
     const int* table; int cols; const int* lengths;
     int n, layer0, n_layers, add_weights;
-    int alone;                                // every unit is one CTA's (filled by the launcher)
+    int alone;                                // CTAs of each unit, a cluster; 0: even split (filled by the launcher)
     // workspace, laid out by the launcher
     float* records;                           // [ranges][2][PARTIAL_FLOATS]
     void* shared;                             // [ranges][2] parts of units shared between ranges

@@ -123,21 +123,37 @@ int main() {
                         walk(valid, cols, shift, layers, hkv, 148, 8, 8);
                         walk(valid, cols, shift, layers, hkv, pick(1, 600), pick(1, 16), pick(1, 16));
                     }
-    // short units: every unit once, its logits in a place of their own inside the workspace
+    // calls of few units: every unit once, its logits in a place of their own inside the workspace,
+    // its blocks split over its CTAs and their warps
     for (int n : {1, 3, 18, 148})
         for (int layers : {1, 2, 28})
             for (int hkv : {1, 2, 4, 8})
-                for (int most : {1, 7, 32}) {
-                    const int units = n * layers * hkv;
+                for (int most : {1, 7, 8, 32, 33, 64, 255, 256, 257, 5000}) {
+                    const int units = n * layers * hkv, ctas = paged_ctas_alone(units, most, 148, 8);
+                    CHECK(ctas == 0 || ctas == 1 || ctas == 2 || ctas == 4);
+                    if (!ctas) continue;
+                    CHECK(units * ctas <= 148 && most <= ctas * 32);
                     std::vector<int> hit(units, 0);
-                    for (int c = 0; c < units; ++c) {
-                        const PagedUnit u = paged_unit_alone(c, n, hkv, most);
+                    for (int i = 0; i < units; ++i) {
+                        const PagedUnit u = paged_unit_alone(i, n, hkv, most);
                         CHECK(u.l >= 0 && u.l < layers && u.b >= 0 && u.b < n && u.kh >= 0 && u.kh < hkv);
-                        CHECK((u.l * n + u.b) * hkv + u.kh == c && u.off == (long long)c * most);
+                        CHECK((u.l * n + u.b) * hkv + u.kh == i && u.off == (long long)i * most);
                         CHECK(u.off + most <= (long long)n * layers * hkv * most);
                         ++hit[(u.l * n + u.b) * hkv + u.kh];
                     }
                     for (int h : hit) CHECK(h == 1);
+                    for (int nblk : {1, 2, most / 2 + 1, most}) {
+                        if (nblk > most) continue;
+                        int at = 0;
+                        for (int r = 0; r < ctas; ++r) {
+                            const int from = nblk * r / ctas, blocks = nblk * (r + 1) / ctas - from;
+                            for (int w = 0; w < 8; ++w) {
+                                CHECK(from + blocks * w / 8 == at);
+                                at = from + blocks * (w + 1) / 8;
+                            }
+                        }
+                        CHECK(at == nblk);
+                    }
                 }
     // places: every combination of bad and good length, sequence, position and page id
     for (int shift = 4; shift <= 9; ++shift) {

@@ -399,8 +399,10 @@ def test_lengths_up_to_the_tables_capacity_and_pages_at_the_pools_ends():
         check_attend(ctx, c, c.query(), add=True)
 
 
-@pytest.mark.parametrize("layers,hkv,n,cols_rows", [(1, 8, 18, 512), (1, 1, 148, 512), (1, 1, 149, 512), (28, 1, 5, 256), (2, 8, 3, 513)])
-def test_short_units_around_the_rule_for_one_cta_each(layers, hkv, n, cols_rows):
+@pytest.mark.parametrize("layers,hkv,n,cols_rows", [(1, 8, 18, 512), (1, 1, 148, 512), (1, 1, 149, 512), (28, 1, 5, 256), (2, 8, 3, 513),
+    (1, 8, 1, 4096), (1, 8, 1, 4097), (1, 4, 2, 4000), (1, 2, 9, 4096), (1, 8, 2, 4096), (1, 8, 3, 2048), (1, 8, 4, 1024),
+    (3, 1, 6, 300), (1, 1, 1, 128), (1, 1, 1, 129), (1, 1, 1, 16)])
+def test_calls_of_few_units_around_the_rule_for_their_own_ctas(layers, hkv, n, cols_rows):
     """Calls on either side of the rule (units and rows that a table can hold), ragged with empty rows."""
     ctx = make(layers, hkv)
     r = np.random.default_rng(n)
