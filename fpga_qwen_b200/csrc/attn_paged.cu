@@ -499,9 +499,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
         }
         if (cnt == nblk) {
             a.out[(size_t)unit * GROUP * D + tid] = o / (head1 ? L[1] : L[0]);
-            if (WEIGHTS) {
+            // the weights of a short unit by one warp, while the others go on to the next unit
+            const bool by_all = cnt > 4 * WARPS;
+            if (WEIGHTS && (by_all || warp == (first >> 1))) {
                 const int lb = unit / hkv, row_l = lb / a.n, row_b = lb - row_l * a.n, row_kh = unit - lb * hkv;
-                add_weights(a, row_l, row_b, row_kh, row_length(a, row_b), 0, cnt, g, M, L, tid, THREADS);
+                add_weights(a, row_l, row_b, row_kh, row_length(a, row_b), 0, cnt, g, M, L, by_all ? tid : lane, by_all ? THREADS : 32);
             }
         } else if (a.alone) {
             joint.o[tid] = o;

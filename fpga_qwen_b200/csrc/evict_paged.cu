@@ -32,7 +32,6 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32;
 constexpr int BINS = 256, BATCH = 4;
 constexpr int SLICE_ROWS = 4096;                   // of a cluster's CTA, where there are SMs for it
 constexpr int MAX_SLICE = 49152;                   // 192 KB of shared memory
@@ -43,7 +42,9 @@ __device__ __forceinline__ int row_length(const PagedEvictArgs& a, int b) {
 }
 
 // The cluster's CTAs each take a contiguous slice of the unit's rows, at most as many as s_w holds.
+template <int SEL_THREADS>
 __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const PagedEvictArgs a) {
+    constexpr int SEL_WARPS = SEL_THREADS / 32;
     extern __shared__ __align__(16) float s_w[];             // the slice's weights
     __shared__ __align__(16) int hist[4][BINS];
     __shared__ __align__(16) int bins[2][BINS];              // of the whole cluster, by turns
@@ -203,10 +204,9 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const PagedEv
     if (ranks > 1) cluster.sync();                           // until the others have read this CTA's memory
 }
 
-constexpr int MOVE_THREADS = 256;
 constexpr int ROW_THREADS = 8, CHUNKS = 16 / ROW_THREADS;    // threads of a row; 16-byte chunks of a thread
 constexpr int PER_THREAD = 2;                                // rows of a thread and tile
-constexpr int MOVE_ROWS = MOVE_THREADS / ROW_THREADS, TILE = MOVE_ROWS * PER_THREAD;
+constexpr int tile_rows(int threads) { return threads / ROW_THREADS * PER_THREAD; }
 
 // Cluster (unit, K|V): moves the kept rows, tile after tile of TILE rows per CTA. Three tiles are
 // under way: one being stored, the next one's rows and the one after's indices and pages being
@@ -214,7 +214,9 @@ constexpr int MOVE_ROWS = MOVE_THREADS / ROW_THREADS, TILE = MOVE_ROWS * PER_THR
 // above those destinations. Rows that are in place already are not touched. Eight threads take a row, two 16-byte chunks each: with
 // sixteen, one chunk each, half of the issue slots went to indices and addresses, which cost a few
 // per cent.
+template <int MOVE_THREADS>
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const PagedEvictArgs a) {
+    constexpr int MOVE_ROWS = MOVE_THREADS / ROW_THREADS, TILE = tile_rows(MOVE_THREADS);
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const int unit = blockIdx.x / ranks, kv = blockIdx.y, tile = TILE * ranks;
@@ -320,13 +322,18 @@ cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t s) {
         ranks *= 2;
     const int per = (max_rows + ranks - 1) / ranks;
     if (per > MAX_SLICE) return cudaErrorInvalidValue;       // (refused before)
-    const cudaError_t e = launch(evict_select_kernel, dim3(units), SEL_THREADS, (size_t)per * sizeof(float), ranks, false, a, s);
+    // short tables: small CTAs, more of them per SM (6,496 units of 65 rows: @@SMALL@@)
+    const bool small = per <= 1024 && ranks == 1;
+    const cudaError_t e = launch(small ? evict_select_kernel<128> : evict_select_kernel<512>, dim3(units), small ? 128 : 512,
+                                 (size_t)per * sizeof(float), ranks, false, a, s);
     if (e != cudaSuccess) return e;
     // move: clusters that fill the GPU (4 CTAs per SM) where the units alone do not and there are rows
-    // for every CTA
+    // for every CTA; where there are many units, CTAs no larger than two tiles of kept rows
     ranks = 1;
-    while (ranks < 16 && units * 2 * ranks * 2 <= 4 * NUM_SMS_B200 && ranks * TILE < a.keep) ranks *= 2;
-    return launch(evict_move_kernel, dim3(units, 2), MOVE_THREADS, 0, ranks, true, a, s);
+    while (ranks < 16 && units * 2 * ranks * 2 <= 4 * NUM_SMS_B200 && ranks * tile_rows(256) < a.keep) ranks *= 2;
+    if (ranks == 1 && a.keep <= 2 * tile_rows(64)) return launch(evict_move_kernel<64>, dim3(units, 2), 64, 0, 1, true, a, s);
+    if (ranks == 1 && a.keep <= 2 * tile_rows(128)) return launch(evict_move_kernel<128>, dim3(units, 2), 128, 0, 1, true, a, s);
+    return launch(evict_move_kernel<256>, dim3(units, 2), 256, 0, ranks, true, a, s);
 }
 
 }  // namespace qattn
