@@ -11,7 +11,7 @@
 //     CTA first scans them. A part can end inside one unit and continue in the next.
 //   * Every warp is its own pipeline from its first block to its last: one lane keeps STAGES blocks
 //     (K and V rows, 8 KB) in flight into the warp's ring with TMA copies (128-byte swizzle),
-//     across unit boundaries, 192 KB per SM. A block never crosses a page, so a block is one page
+//     across unit boundaries, 128 KB per SM. A block never crosses a page, so a block is one page
 //     id; the next id is loaded one block ahead. No barrier between the warps until all are
 //     done: a unit inside a warp's part is finished by the warp alone.
 //   * Few instructions per block. With FP32 FMAs a block of 16 rows took about 560 warp
@@ -26,8 +26,9 @@
 // each the sum of two FP16 halves: 22 bits, or 2^-38 of the largest, whichever is coarser; sums are
 // FP32, and long sums are made by FADD: the tensor core's own accumulation truncates, which over the
 // hundred blocks of a long history costs a few 2^-20 (2.0e-6 off in 2-norm against 64 bits at
-// 131071 rows), so it takes no more than two steps of a chain. The high half is rounded towards zero and neither half of a nonzero value is zero, so
-// both have its sign and an infinite key or value gives what the formula gives.
+// 131071 rows), so it takes no more than two steps of a chain. The high half is rounded towards zero and
+// neither half of a nonzero value is zero, so both have its sign and an infinite key or value gives
+// what the formula gives.
 //
 // A unit that several warps of a CTA share is merged through shared memory at the CTA's end; a
 // unit that several CTAs share leaves one record (max, sum, 2 x 128 partial output) per CTA, and a

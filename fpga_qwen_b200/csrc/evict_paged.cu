@@ -211,9 +211,9 @@ constexpr int tile_rows(int threads) { return threads / ROW_THREADS * PER_THREAD
 // Cluster (unit, K|V): moves the kept rows, tile after tile of TILE rows per CTA. Three tiles are
 // under way: one being stored, the next one's rows and the one after's indices and pages being
 // loaded. A tile's rows may be loaded before the tile before it is stored, since its sources lie
-// above those destinations. Rows that are in place already are not touched. Eight threads take a row, two 16-byte chunks each: with
-// sixteen, one chunk each, half of the issue slots went to indices and addresses, which cost a few
-// per cent.
+// above those destinations. Rows that are in place already are not touched. Eight threads take a
+// row, two 16-byte chunks each: with sixteen, one chunk each, half of the issue slots went to indices
+// and addresses, which cost a few per cent.
 template <int MOVE_THREADS>
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const PagedEvictArgs a) {
     constexpr int MOVE_ROWS = MOVE_THREADS / ROW_THREADS, TILE = tile_rows(MOVE_THREADS);

@@ -1653,6 +1653,7 @@ int qa_paged_attn(qa_ctx* ctx, const qa_pages* pages, const int* table, int tabl
     c.inputs_read_once = decode_inputs_read_once(n_layers, n, ctx->hkv);
     return run_call(ctx, -1, layer, n_layers, c, [&](int l0, int nl, const float* const* din, float* const* dout) {
         a.q = din[0]; a.out = dout[0]; a.layer0 = l0; a.n_layers = nl;
+        ctx->last_fused_step = false;
         const cudaError_t e = launch_paged_attn(a, map, workspace, ctx->stream);
         if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, e, "paged_attn"); }
         return after_launch(ctx, -1, "paged_attn");
@@ -1678,6 +1679,7 @@ int qa_paged_evict(qa_ctx* ctx, const qa_pages* pages, const int* src_table, int
     a.src_table = src_table; a.src_cols = src_cols; a.dst_table = dst_table; a.dst_cols = dst_cols;
     a.lengths = lengths; a.new_lengths = new_lengths; a.n = n; a.keep = keep; a.recent = recent; a.kept = kept;
     a.error = ctx->error;
+    ctx->last_fused_step = false;
     const cudaError_t e = launch_paged_evict(a, ctx->stream);
     if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, e, "paged_evict"); }
     return after_launch(ctx, -1, "paged_evict");

@@ -154,7 +154,8 @@ class PagedSequences:
 
     # -- prompts -------------------------------------------------------------------------------
     def prefill(self, seq: int, q, k, v):
-        """A prompt of n rows for a new sequence; returns its attention outputs [L][n][hq][128]."""
+        """A prompt of n rows for a new sequence; returns its attention outputs [L][n][hq][128]. The
+        sequence takes part in steps from the next begin_step on."""
         n = q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 4 else 0
         self.host._check(seq)
         if self.host.rows[seq] or self.host.position[seq]:
@@ -165,16 +166,14 @@ class PagedSequences:
             raise QAttnError(QA_ERR_CAPACITY, "Context capacity exceeded")
         self._check_inputs(n, self.layers, q=q, k=k, v=v)
         self._grow({seq: n})
-        self._stream()
-        qn, out = torch.empty_like(q), torch.empty_like(q)
         try:
+            self._stream()
+            qn, out = torch.empty_like(q), torch.empty_like(q)
             self._run_prompt(seq, n, q, k, v, qn, out)
-        except QAttnError:
+        except Exception:
             self.host.shrink(seq, 0)                     # as an execution failure resets a slot's sequence
             self.host.position[seq] = 0
-            self.lengths[seq] = 0
             raise
-        self.lengths[seq], self.positions[seq] = n, n - 1
         return out
 
     def _run_prompt(self, seq, n, q, k, v, qn, out):
@@ -237,9 +236,11 @@ class PagedSequences:
         keep = min(keep, self.host.cols * self.host.page_rows)
         recent = min(recent, keep)
         kept = torch.empty(n, self.layers, self.ctx.hkv, keep, dtype=torch.int32, device=self.table.device)
+        rows = self._int32(self.host.rows)               # (lengths leaves out prompts since the last begin_step)
         self._stream()
         self.ctx.paged_evict(self.pages, self.table.data_ptr(), self.host.cols, self.table.data_ptr(), self.host.cols,
-                             self.lengths.data_ptr(), self.lengths.data_ptr(), n, keep, recent, kept.data_ptr())
+                             rows.data_ptr(), rows.data_ptr(), n, keep, recent, kept.data_ptr())
+        self.lengths.copy_(torch.minimum(self.lengths, rows))
         for seq in self.host.live():
             self.host.shrink(seq, min(self.host.rows[seq], keep))
         return kept

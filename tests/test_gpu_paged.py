@@ -326,6 +326,68 @@ def test_attention_is_reproducible_and_graph_replays_with_new_lengths():
     ctx.sync()
 
 
+@pytest.mark.parametrize("lengths,layers", [([200, 300], 1), ([1000, 900], 1), ([300, 0, 2000], 4)])    # one CTA a unit, clusters, even split
+def test_captured_calls_between_forked_streams(lengths, layers):
+    """Inputs written by two streams that join before the calls, results read by two that fork behind them,
+    all in one graph: every replay sees its own inputs, and its readers all its results."""
+    ctx = make(layers, 8)
+    n, keep = len(lengths), 64
+    c = Cache(lengths, layers, 8, seed=61)
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    main.wait_stream(torch.cuda.current_stream())
+    ctx.set_stream(main.cuda_stream)
+    size = ctx.paged_workspace(n, layers, c.cols * c.page, True)
+    with torch.cuda.stream(main):
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        q_new, lens_new, kv_new, w_new = c.query(), i32(lengths), c.kv.clone(), c.w.clone()
+        q, lens, out = torch.zeros_like(q_new), i32([0] * n), torch.empty_like(q_new)
+        out_seen, w_seen, kv_seen = torch.empty_like(out), torch.empty_like(c.w), torch.empty_like(c.kv)
+        new, kept = i32([0] * n), torch.empty(n, layers, 8, keep, dtype=torch.int32, device="cuda")
+        kept_seen, new_seen = torch.empty_like(kept), torch.empty_like(new)
+
+        def calls():
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                c.kv.copy_(kv_new)
+                lens.copy_(lens_new)
+            q.copy_(q_new)
+            c.w.copy_(w_new)
+            main.wait_stream(side)
+            ctx.paged_attn(c.pages, c.table.data_ptr(), c.cols, lens.data_ptr(), n, 0, layers, q.data_ptr(), out.data_ptr(),
+                           True, ws.data_ptr(), size)
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                out_seen.copy_(out)
+            w_seen.copy_(c.w)
+            ctx.paged_evict(c.pages, c.table.data_ptr(), c.cols, c.table.data_ptr(), c.cols, lens.data_ptr(), new.data_ptr(),
+                            n, keep, 16, kept.data_ptr())
+            main.wait_stream(side)
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                kept_seen.copy_(kept)
+                new_seen.copy_(new)
+            kv_seen.copy_(c.kv)
+            main.wait_stream(side)
+        main.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=main):
+            calls()
+        seen = (out_seen, w_seen, kv_seen, kept_seen, new_seen)
+        for i in range(12):
+            q_new.copy_(c.query())
+            lens_new.copy_(i32([max(m - 37 * i, 0) for m in lengths]))
+            for t in seen:
+                t.zero_()
+            graph.replay()
+            got = [t.clone() for t in seen]
+            calls()
+            main.synchronize()
+            for x, y in zip(got, seen):
+                assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+            assert bool(out_seen[:, 0].any()) == (lens_new[0] > 0) and new_seen.tolist() == [min(m, keep) for m in lens_new.tolist()]
+    ctx.sync()
+
+
 def test_calls_on_two_streams_with_their_own_workspaces():
     ctx = make(2, 8)
     c = Cache([3000, 1500], 2, 8, page=64, seed=13)
@@ -1017,4 +1079,44 @@ def test_sequences_captured_steps_stay_valid_and_shapes_are_checked():
     one.attend(qn[1:], 1)
     with pytest.raises(qattn.QAttnError):
         one.attend(qn)                                  # its workspace holds one layer
+    ctx.sync()
+
+
+def test_sequences_prefilled_within_a_step_join_at_the_next():
+    """A prompt that arrives between begin_step and append is no part of the step: the step writes no row of
+    it and gives zeros; an eviction sees all its rows, and the next step appends behind them."""
+    from fpga_qwen_b200.paged import PagedSequences
+    L, hkv = 2, 2
+    ctx = make(L, hkv, context=128)
+    s = PagedSequences(ctx, n_pages=40, page_rows=16, max_seqs=3, max_rows=128)
+    g = torch.Generator("cuda").manual_seed(11)
+
+    def draw(n):
+        return [torch.randn(L, n, h, D, device="cuda", generator=g) for h in (4, 2, 2)]
+
+    def cached(seq):
+        t = torch.arange(s.rows(seq), device="cuda")
+        return s.kv[s.table[seq].long()[t // 16], :, :, :, t % 16].clone()
+    s.prefill(s.open(), *draw(20))
+    s.begin_step()
+    late = s.open()
+    s.prefill(late, *draw(50))
+    before = cached(late)
+    out = s.attend(s.append(*draw(3)))
+    assert torch.equal(before.view(torch.int16), cached(late).view(torch.int16))
+    assert out[:, 0].all() and not out[:, 1:].any()
+    third = s.open()
+    s.prefill(third, *draw(40))
+    kept = s.evict(32, 8)
+    # the prompt's rows weigh nothing yet: the lowest 24 and the last 8
+    assert kept[late].tolist() == [[list(range(24)) + list(range(42, 50))] * hkv] * L
+    assert kept[third].tolist() == [[list(range(24)) + list(range(32, 40))] * hkv] * L
+    assert [s.rows(b) for b in range(3)] == [21, 32, 32] and s.lengths.tolist() == [21, 0, 0]
+    s.begin_step()
+    assert s.lengths.tolist() == [22, 33, 33] and s.positions.tolist() == [21, 50, 40]
+    out = s.attend(s.append(*draw(3)))
+    assert out.all()
+    after = cached(late)
+    assert torch.equal(after[:24].view(torch.int16), before[:24].view(torch.int16))
+    assert torch.equal(after[24:32].view(torch.int16), before[42:].view(torch.int16))
     ctx.sync()
