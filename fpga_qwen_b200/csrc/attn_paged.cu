@@ -48,7 +48,10 @@
 // four, of its own, without the scan of the lengths, and a cluster's CTAs join their parts over
 // distributed shared memory, without the second launch (paged_ctas_alone says when: 8 units of 256
 // rows 8.6 -> 5.9 us, of 1024 rows 9.0 -> 8.0 us, 32 units of 2048 rows 13.7 -> 10.6 us, 144 units
-// of 512 rows 13.7 -> 8.4 us).
+// of 512 rows 13.7 -> 8.4 us). Neither do calls of one sequence, long or not, whose units are equally
+// long: up to 148 of them have CTAs of their own, up to 296 half-size CTAs, two per SM
+// (paged_alone_equal: 224 units of 3970 rows 75.1 -> 68.5 us, 6.6 TB/s; with weights, of 2049 rows
+// 50.3 -> 42.0 us; 112 units of 8192 rows 78.1 -> 71.7 us).
 //
 // Every wait is bounded: on expiry the CTA records an error code, consumes no further block, and
 // drains its copies before it exits.
@@ -68,7 +71,7 @@ constexpr int BLK = PAGED_BLK;
 constexpr int STAGES = 2;                     // blocks in flight per warp
 constexpr int HALF_STAGE = BLK * D * 2;       // K rows, then V rows of a block: 4 KB each, [channel half][row][64]
 constexpr int STAGE = 2 * HALF_STAGE;
-constexpr int RING = WARPS * STAGES * STAGE;
+constexpr int ring_bytes(int warps) { return warps * STAGES * STAGE; }
 constexpr int CTAS = NUM_SMS_B200;            // ranges
 constexpr int MIN_BLOCKS = WARPS;             // blocks per range, at least
 constexpr int JOIN_THREADS = 256, JOIN_GROUPS = JOIN_THREADS / (GROUP * D / 4);
@@ -193,47 +196,49 @@ __device__ __forceinline__ uint32_t split_half(float x) {
     return hi | lo << 16;
 }
 
-template <bool WEIGHTS>
-__global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap map) {
-    extern __shared__ __align__(1024) uint8_t ring[];        // [WARPS][STAGES][K rows | V rows]
-    __shared__ __align__(8) uint64_t full[WARPS][STAGES];
+// W warps: WARPS, or fewer for calls whose units each have one CTA (a.alone == 1).
+template <bool WEIGHTS, int W = WARPS>
+__global__ void __launch_bounds__(W * 32, 1) attn_paged_split_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap map) {
+    extern __shared__ __align__(1024) uint8_t ring[];        // [W][STAGES][K rows | V rows]
+    constexpr int T = W * 32;
+    __shared__ __align__(8) uint64_t full[W][STAGES];
     __shared__ int start[MAX_PAGED_BATCH + 1];
     __shared__ int warp_sum[WARPS];
-    __shared__ Part parts[WARPS][2];                         // [0]: of the warp's first unit, [1]: of its last
-    __shared__ __align__(16) float s_part[WARPS][2][GROUP * D];
+    __shared__ Part parts[W][2];                             // [0]: of the warp's first unit, [1]: of its last
+    __shared__ __align__(16) float s_part[W][2][GROUP * D];
     __shared__ Joint joint;
     __shared__ int abort_flag, never_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
     const int g8 = lane >> 2, j4 = lane & 3, head = j4 & 1;  // tile row or column, and the column pair's head
-    const int hkv = a.kv.hkv;
+    const int hkv = a.kv.hkv, alone = W < WARPS ? 1 : a.alone;
     if (tid == 0) {
         abort_flag = 0; never_abort = 0; joint.cnt = 0;
-        for (int i = 0; i < WARPS * STAGES; ++i) mbar_init(&full[0][0] + i, 1);
+        for (int i = 0; i < W * STAGES; ++i) mbar_init(&full[0][0] + i, 1);
         fence_mbar_init();
         prefetch_tmap(&map);
     }
-    if (tid < WARPS * 2) parts[tid >> 1][tid & 1].unit = -1;
+    if (tid < W * 2) parts[tid >> 1][tid & 1].unit = -1;
     // What ran before is complete. (No read-only loads below: they may move across this, and what it
     // waits for may write the queries, tables and lengths.)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     PagedSplit sp{};
-    PagedUnit only{};                                        // a.alone: the CTA's unit
+    PagedUnit only{};                                        // alone: the CTA's unit
     long long c_begin;
     int c_blocks;                                            // at most 2^28 (64 layers, 8 heads, 2^30 rows over 148 ranges)
-    if (a.alone) {
-        const int i = c / a.alone, rank = c - i * a.alone;   // the CTA's unit, and its place in the cluster
+    if (alone) {
+        const int i = c / alone, rank = c - i * alone;       // the CTA's unit, and its place in the cluster
         only = paged_unit_alone(i, a.n, hkv, ((a.cols << a.kv.shift) + BLK - 1) / BLK);
         const int given = a.lengths[only.b], len = paged_length(given, a.cols, a.kv.shift);
         if (given != len && tid == 0) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
         only.nblk = (len + BLK - 1) / BLK;
         if (len == 0) {                                      // (for the whole cluster)
-            if (rank == 0) a.out[(size_t)i * GROUP * D + tid] = 0.f;
+            for (int col = tid; rank == 0 && col < GROUP * D; col += T) a.out[(size_t)i * GROUP * D + col] = 0.f;
             return;
         }
-        const int from = only.nblk * rank / a.alone;
+        const int from = only.nblk * rank / alone;
         c_begin = only.off + from;
-        c_blocks = only.nblk * (rank + 1) / a.alone - from;
+        c_blocks = only.nblk * (rank + 1) / alone - from;
         __syncthreads();                                     // the barriers and parts above are ready
     } else {
         sp = scan_lengths(a, start, warp_sum);               // (its barriers cover them too)
@@ -244,9 +249,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
         c_begin = sp.begin(c);
         c_blocks = (int)(sp.begin(c + 1) - c_begin);
     }
-    auto unit_of = [&](long long g) { return a.alone ? only : paged_unit_of(start, a.n, hkv, g); };
+    auto unit_of = [&](long long g) { return alone ? only : paged_unit_of(start, a.n, hkv, g); };
     // this warp's blocks [g_begin, g_end) of the range
-    const long long g_begin = c_begin + c_blocks * warp / WARPS, g_end = c_begin + c_blocks * (warp + 1) / WARPS;
+    const long long g_begin = c_begin + c_blocks * warp / W, g_end = c_begin + c_blocks * (warp + 1) / W;
     const float qscale = 1.4426950408889634f * 0.08838834764831845f;   // log2(e)/sqrt(128)
     const int mask = (1 << a.kv.shift) - 1;
     uint8_t* const my_ring = ring + warp * (STAGES * STAGE);
@@ -467,9 +472,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
 
     // ---- merge the warps' parts: those of one unit are neighbours in the order of the blocks ----
     // every warp holds all parts, two lanes each: lane is part lane % 16 and head lane / 16
-    static_assert(WARPS * 2 == 16, "two heads of all parts fill a warp");
+    static_assert(W * 2 <= 16 && GROUP * D % T == 0, "two heads of all parts within a warp; whole rounds of columns");
     const int part = lane & 15, part_head = lane >> 4;
-    const Part p = parts[part >> 1][part & 1];
+    Part p{};
+    p.unit = -1;
+    if (part < W * 2) p = parts[part >> 1][part & 1];
     const float p_m = part_head ? p.m[1] : p.m[0], p_l = part_head ? p.l[1] : p.l[0];
     unsigned left = __ballot_sync(0xffffffffu, p.unit >= 0) & 0xffff;
     unsigned have = 0;                                       // records of this range
@@ -491,30 +498,39 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
         for (int x = 8; x >= 1; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
         const float M[GROUP] = {__shfl_sync(0xffffffffu, top, 0), __shfl_sync(0xffffffffu, top, 16)};
         const float L[GROUP] = {__shfl_sync(0xffffffffu, sum, 0), __shfl_sync(0xffffffffu, sum, 16)};
-        const bool head1 = tid >= D;                         // (a warp's columns are of one head)
-        float o = 0.f;
+        constexpr int COLS = GROUP * D / T;                  // of a thread, T apart
+        float o[COLS];
         #pragma unroll
-        for (int k = 0; k < WARPS * 2; ++k) {
-            const float fk = __shfl_sync(0xffffffffu, f, k + (head1 ? 16 : 0));
-            if (group >> k & 1) o += fk * s_part[k >> 1][k & 1][tid];
+        for (int x = 0; x < COLS; ++x) {
+            const int col = x * T + tid;
+            o[x] = 0.f;
+            #pragma unroll
+            for (int k = 0; k < W * 2; ++k) {
+                const float fk = __shfl_sync(0xffffffffu, f, k + (col >= D ? 16 : 0));   // (a warp's columns are of one head)
+                if (group >> k & 1) o[x] += fk * s_part[k >> 1][k & 1][col];
+            }
         }
         if (cnt == nblk) {
-            a.out[(size_t)unit * GROUP * D + tid] = o / (head1 ? L[1] : L[0]);
+            #pragma unroll
+            for (int x = 0; x < COLS; ++x)
+                a.out[(size_t)unit * GROUP * D + x * T + tid] = o[x] / (x * T + tid >= D ? L[1] : L[0]);
             // the weights of a short unit by one warp, while the others go on to the next unit
-            const bool by_all = cnt > 4 * WARPS;
+            const bool by_all = cnt > 4 * W;
             if (WEIGHTS && (by_all || warp == (first >> 1))) {
                 const int lb = unit / hkv, row_l = lb / a.n, row_b = lb - row_l * a.n, row_kh = unit - lb * hkv;
-                add_weights(a, row_l, row_b, row_kh, row_length(a, row_b), 0, cnt, g, M, L, by_all ? tid : lane, by_all ? THREADS : 32);
+                add_weights(a, row_l, row_b, row_kh, row_length(a, row_b), 0, cnt, g, M, L, by_all ? tid : lane, by_all ? T : 32);
             }
-        } else if (a.alone) {
-            joint.o[tid] = o;
+        } else if (alone) {
+            #pragma unroll
+            for (int x = 0; x < COLS; ++x) joint.o[x * T + tid] = o[x];
             if (tid < GROUP) { joint.m[tid] = tid ? M[1] : M[0]; joint.l[tid] = tid ? L[1] : L[0]; }
             if (tid == 0) joint.cnt = cnt;
         } else {
             const int slot = g != c_begin;
             float* rec = a.records + ((size_t)c * 2 + slot) * PARTIAL_FLOATS;
             if (tid < GROUP) { rec[tid] = M[tid]; rec[GROUP + tid] = L[tid]; }
-            rec[4 + tid] = o;
+            #pragma unroll
+            for (int x = 0; x < COLS; ++x) rec[4 + x * T + tid] = o[x];
             if (tid == slot * 32) {
                 const long long off = g - blk0;
                 Shared s;
@@ -527,11 +543,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
             have |= 1u << slot;
         }
     }
-    if (!a.alone) {
+    if (!alone) {
         if (tid < 2 && !(have >> tid & 1)) shared_of(a)[c * 2 + tid].nrec = 0;
         return;
     }
-    if (a.alone == 1) return;
+    if (alone == 1) return;
     // ---- join the cluster's parts (none where one CTA held the whole unit) ----
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
@@ -541,7 +557,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
     for (int r = 0; r < 4; ++r) {
         cnts[r] = 0;
         f[r][0] = f[r][1] = -INFINITY;
-        if (r >= a.alone) continue;
+        if (r >= alone) continue;
         const Joint* x = cluster.map_shared_rank(&joint, r);
         cnts[r] = x->cnt;
         f[r][0] = x->m[0]; f[r][1] = x->m[1];
@@ -565,8 +581,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_paged_split_kernel(const Page
             }
             sum += (tid < D ? f[r][0] : f[r][1]) * x->o[tid];
         }
-        const int i = c / a.alone;
-        if (c - i * a.alone == 0) a.out[(size_t)i * GROUP * D + tid] = sum / (tid < D ? L[0] : L[1]);
+        const int i = c / alone;
+        if (c - i * alone == 0) a.out[(size_t)i * GROUP * D + tid] = sum / (tid < D ? L[0] : L[1]);
         if (WEIGHTS && c_blocks)
             add_weights(a, only.l, only.b, only.kh, row_length(a, only.b), (int)(c_begin - only.off), c_blocks, c_begin, M, L, tid, THREADS);
     }
@@ -678,10 +694,11 @@ static cudaError_t launch_dependent(void (*kernel)(Params...), int ctas, int clu
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <bool WEIGHTS>
+template <bool WEIGHTS, int W>
 static cudaError_t launch_split(const PagedAttnArgs& a, const CUtensorMap& map, int ctas, cudaStream_t s) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_paged_split_kernel<WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING);
-    return e != cudaSuccess ? e : launch_dependent(attn_paged_split_kernel<WEIGHTS>, ctas, a.alone > 1 ? a.alone : 1, THREADS, RING, s, a, map);
+    const auto kernel = attn_paged_split_kernel<WEIGHTS, W>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_bytes(W));
+    return e != cudaSuccess ? e : launch_dependent(kernel, ctas, a.alone > 1 ? a.alone : 1, W * 32, ring_bytes(W), s, a, map);
 }
 
 cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* workspace, cudaStream_t s) {
@@ -690,9 +707,17 @@ cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* wor
     a.shared = ws + RECORD_BYTES;
     a.logits = reinterpret_cast<float*>(ws + RECORD_BYTES + SHARED_BYTES);
     const long long units = (long long)a.n * a.n_layers * a.kv.hkv;
-    a.alone = paged_ctas_alone(units, ((a.cols << a.kv.shift) + BLK - 1) / BLK, CTAS, WARPS);
+    const int most = ((a.cols << a.kv.shift) + BLK - 1) / BLK;
+    int warps = WARPS;
+    if (a.n > 1) a.alone = paged_ctas_alone(units, most, CTAS, WARPS);
+    else {
+        const PagedAlone p = paged_alone_equal(units, most, CTAS, WARPS);
+        a.alone = p.ctas;
+        warps = p.warps;
+    }
     const int ctas = a.alone ? (int)units * a.alone : CTAS;
-    const cudaError_t e = a.add_weights ? launch_split<true>(a, map, ctas, s) : launch_split<false>(a, map, ctas, s);
+    const cudaError_t e = warps == WARPS ? a.add_weights ? launch_split<true, WARPS>(a, map, ctas, s) : launch_split<false, WARPS>(a, map, ctas, s)
+                                         : a.add_weights ? launch_split<true, WARPS / 2>(a, map, ctas, s) : launch_split<false, WARPS / 2>(a, map, ctas, s);
     return e != cudaSuccess || a.alone ? e : launch_dependent(attn_paged_join_kernel, CTAS * 2, 1, JOIN_THREADS, 0, s, a);
 }
 

@@ -155,6 +155,31 @@ int main() {
                         CHECK(at == nblk);
                     }
                 }
+    // calls of one sequence: CTAs that fit the GPU at once (two per SM where they have half the warps), and the
+    // same split of a unit's blocks over them and their warps
+    for (int layers = 1; layers <= 64; ++layers)
+        for (int hkv : {1, 2, 4, 8})
+            for (int most : {1, 2, 7, 8, 31, 32, 33, 64, 129, 249, 256, 513, 8192, 65536}) {
+                const int units = layers * hkv;
+                const PagedAlone p = paged_alone_equal(units, most, 148, 8);
+                CHECK((p.ctas == 0 && p.warps == 8) || (p.warps == 8 && (p.ctas == 1 || p.ctas == 2 || p.ctas == 4) && units * p.ctas <= 148) ||
+                      (p.warps == 4 && p.ctas == 1 && units <= 296));
+                CHECK(p.ctas != 4 || units * 4 <= 128);
+                CHECK(units > 148 || most > 8 || p.ctas == 1);
+                CHECK(units <= 296 || p.ctas == 0);
+                if (p.ctas == 0) continue;
+                for (int nblk : {1, most / 2 + 1, most}) {
+                    int at = 0;
+                    for (int k = 0; k < p.ctas; ++k) {
+                        const int from = nblk * k / p.ctas, blocks = nblk * (k + 1) / p.ctas - from;
+                        for (int w = 0; w < p.warps; ++w) {
+                            CHECK(from + blocks * w / p.warps == at);
+                            at = from + blocks * (w + 1) / p.warps;
+                        }
+                    }
+                    CHECK(at == nblk);
+                }
+            }
     // places: every combination of bad and good length, sequence, position and page id
     for (int shift = 4; shift <= 9; ++shift) {
         const int cols = 3, n_seqs = 4, n_pages = 7;

@@ -485,6 +485,25 @@ def test_calls_of_few_units_around_the_rule_for_their_own_ctas(layers, hkv, n, c
     assert bool(((out.double() - want).abs() <= tol)[:, 1:].all())
 
 
+@pytest.mark.parametrize("layers,hkv,rows", [(28, 8, 3970), (28, 8, 1), (28, 8, 63), (28, 8, 65), (37, 8, 500), (38, 8, 40), (19, 8, 1000), (64, 4, 17),
+    (40, 4, 1024), (40, 4, 1600), (28, 4, 2049), (28, 4, 15), (28, 2, 1500), (28, 1, 3000), (2, 8, 1537), (37, 4, 4100)])
+def test_one_sequence_of_many_layers(layers, hkv, rows):
+    """One sequence: CTAs, half-size CTAs or clusters for every layer and KV head, whatever the rows; empty
+    and too long lengths."""
+    ctx = make(layers, hkv)
+    c = Cache([rows], layers, hkv, page=16, seed=rows, extra_cols=0)
+    q = c.query()
+    check_attend(ctx, c, q, add=True)
+    out = check_attend(ctx, c, q)
+    assert torch.equal(out, attend(ctx, c, q))
+    assert not attend(ctx, c, q, lengths=i32([0])).any()
+    ctx.sync()
+    assert not attend(ctx, c, q, lengths=i32([c.cols * 16 + 1])).any()
+    with pytest.raises(qattn.QAttnError) as err:
+        ctx.sync()
+    assert "code 61" in str(err.value)
+
+
 # ---- append --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("hkv,page,n", [(8, 16, 1), (8, 16, 5), (4, 32, 7), (2, 64, 33), (1, 512, 130), (8, 128, 40)])
 def test_append_tokens_bit_exact_with_the_oracle(hkv, page, n):
