@@ -75,6 +75,7 @@ constexpr int ring_bytes(int warps) { return warps * STAGES * STAGE; }
 constexpr int CTAS = NUM_SMS_B200;            // ranges
 constexpr int MIN_BLOCKS = WARPS;             // blocks per range, at least
 constexpr int JOIN_THREADS = 256, JOIN_GROUPS = JOIN_THREADS / (GROUP * D / 4);
+constexpr int JOIN_PARTS = 3;
 constexpr int WAIT_CODE = 43;                 // error code of an expired wait
 
 // A part of a unit that its worker does not finish alone.
@@ -590,18 +591,21 @@ __global__ void __launch_bounds__(W * 32, 1) attn_paged_split_kernel(const Paged
 }
 
 // CTA (range c, side): if c is the first range of the side's shared unit, joins the unit; with weights,
-// adds those of the range's part of it. Beside that, before the first launch is done: rows of
-// length 0. (One CTA per side rather than one after the other: the chain of latencies is short.)
+// adds those of the range's part of it, shared with JOIN_PARTS - 1 more CTAs (2 rows of 131071 and
+// 77777: 162.5 -> 158.2 us; no slower where there is little to add). Beside that, before the first
+// launch is done: rows of length 0. (One CTA per side rather than one after the other: the chain of
+// latencies is short.)
 __global__ void __launch_bounds__(JOIN_THREADS, 5) attn_paged_join_kernel(const PagedAttnArgs a) {
     __shared__ float s_f[CTAS][GROUP];                       // factor of each record
     __shared__ float red[2 * GROUP][JOIN_THREADS / 32];
     __shared__ __align__(16) float s_sum[JOIN_GROUPS][GROUP * D];
     static_assert(CTAS <= JOIN_THREADS && GROUP * D == JOIN_THREADS, "one record, and one column, a thread");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x >> 1;
+    const int part = blockIdx.y;
     const int row_floats = GROUP * a.kv.hkv * D;
-    for (int b = tid; b < a.n && blockIdx.x == 0; b += JOIN_THREADS)
+    for (int b = tid; b < a.n && blockIdx.x + part == 0; b += JOIN_THREADS)
         if (a.lengths[b] != row_length(a, b)) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
-    for (int i = blockIdx.x; i < a.n_layers * a.n; i += gridDim.x)
+    for (int i = blockIdx.x; part == 0 && i < a.n_layers * a.n; i += gridDim.x)
         if (row_length(a, i % a.n) == 0)
             for (int j = tid * 4; j < row_floats; j += JOIN_THREADS * 4)
                 *reinterpret_cast<float4*>(a.out + (size_t)i * row_floats + j) = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -644,7 +648,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, 5) attn_paged_join_kernel(const 
         #pragma unroll
         for (int w = 0; w < JOIN_THREADS / 32; ++w) L[k] += red[GROUP + k][w];
     }
-    if (s.first == c) {
+    if (s.first == c && part == 0) {
         // four columns a thread, every fourth record a group, then the groups in order
         const int grp = tid / (GROUP * D / 4), col = tid % (GROUP * D / 4) * 4;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -663,7 +667,8 @@ __global__ void __launch_bounds__(JOIN_THREADS, 5) attn_paged_join_kernel(const 
     }
     if (a.add_weights) {
         const int lb = s.unit / a.kv.hkv, b = lb % a.n;
-        add_weights(a, lb / a.n, b, s.unit % a.kv.hkv, row_length(a, b), s.blk0, s.cnt, s.g, M, L, tid, JOIN_THREADS);
+        add_weights(a, lb / a.n, b, s.unit % a.kv.hkv, row_length(a, b), s.blk0, s.cnt, s.g, M, L, part * JOIN_THREADS + tid,
+                    JOIN_PARTS * JOIN_THREADS);
     }
 }
 
@@ -681,10 +686,10 @@ size_t paged_attn_workspace(int n, int n_layers, int hkv, int max_rows, bool wei
 
 // A launch whose CTAs may start while the launch before it ends; they wait for its end themselves.
 template <class... Params, class... Args>
-static cudaError_t launch_dependent(void (*kernel)(Params...), int ctas, int cluster, int threads, size_t smem, cudaStream_t s,
+static cudaError_t launch_dependent(void (*kernel)(Params...), dim3 ctas, int cluster, int threads, size_t smem, cudaStream_t s,
                                     const Args&... args) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cfg.gridDim = ctas; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
     cudaLaunchAttribute attr[2]{};
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -718,7 +723,7 @@ cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* wor
     const int ctas = a.alone ? (int)units * a.alone : CTAS;
     const cudaError_t e = warps == WARPS ? a.add_weights ? launch_split<true, WARPS>(a, map, ctas, s) : launch_split<false, WARPS>(a, map, ctas, s)
                                          : a.add_weights ? launch_split<true, WARPS / 2>(a, map, ctas, s) : launch_split<false, WARPS / 2>(a, map, ctas, s);
-    return e != cudaSuccess || a.alone ? e : launch_dependent(attn_paged_join_kernel, CTAS * 2, 1, JOIN_THREADS, 0, s, a);
+    return e != cudaSuccess || a.alone ? e : launch_dependent(attn_paged_join_kernel, dim3(CTAS * 2, a.add_weights ? JOIN_PARTS : 1), 1, JOIN_THREADS, 0, s, a);
 }
 
 }  // namespace qattn
