@@ -684,15 +684,15 @@ size_t paged_attn_workspace(int n, int n_layers, int hkv, int max_rows, bool wei
     return RECORD_BYTES + SHARED_BYTES + (weights ? blocks * BLK * 2 * sizeof(float) : 0);
 }
 
-// A launch whose CTAs may start while the launch before it ends; they wait for its end themselves.
+// With `overlap` the CTAs may start while the launch before this one ends; they wait for its end themselves.
 template <class... Params, class... Args>
-static cudaError_t launch_dependent(void (*kernel)(Params...), dim3 ctas, int cluster, int threads, size_t smem, cudaStream_t s,
-                                    const Args&... args) {
+static cudaError_t launch(void (*kernel)(Params...), bool overlap, dim3 ctas, int cluster, int threads, size_t smem, cudaStream_t s,
+                          const Args&... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = ctas; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
     cudaLaunchAttribute attr[2]{};
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].val.programmaticStreamSerializationAllowed = overlap;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
@@ -703,7 +703,7 @@ template <bool WEIGHTS, int W>
 static cudaError_t launch_split(const PagedAttnArgs& a, const CUtensorMap& map, int ctas, cudaStream_t s) {
     const auto kernel = attn_paged_split_kernel<WEIGHTS, W>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_bytes(W));
-    return e != cudaSuccess ? e : launch_dependent(kernel, ctas, a.alone > 1 ? a.alone : 1, W * 32, ring_bytes(W), s, a, map);
+    return e != cudaSuccess ? e : launch(kernel, a.overlap, ctas, a.alone > 1 ? a.alone : 1, W * 32, ring_bytes(W), s, a, map);
 }
 
 cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* workspace, cudaStream_t s) {
@@ -723,7 +723,7 @@ cudaError_t launch_paged_attn(PagedAttnArgs a, const CUtensorMap& map, void* wor
     const int ctas = a.alone ? (int)units * a.alone : CTAS;
     const cudaError_t e = warps == WARPS ? a.add_weights ? launch_split<true, WARPS>(a, map, ctas, s) : launch_split<false, WARPS>(a, map, ctas, s)
                                          : a.add_weights ? launch_split<true, WARPS / 2>(a, map, ctas, s) : launch_split<false, WARPS / 2>(a, map, ctas, s);
-    return e != cudaSuccess || a.alone ? e : launch_dependent(attn_paged_join_kernel, dim3(CTAS * 2, a.add_weights ? JOIN_PARTS : 1), 1, JOIN_THREADS, 0, s, a);
+    return e != cudaSuccess || a.alone ? e : launch(attn_paged_join_kernel, true, dim3(CTAS * 2, a.add_weights ? JOIN_PARTS : 1), 1, JOIN_THREADS, 0, s, a);
 }
 
 }  // namespace qattn

@@ -111,6 +111,7 @@ struct qa_ctx {
     std::vector<int> pool_chunk;
     bool step_overlap = false;             // qa_set_step_overlap
     bool last_fused_step = false;          // the last launch on the stream was a fused decode step
+    bool last_gather_wait = false;         // it was a gather's wait, which may end before the step in front of it
     size_t step_out_bytes = 0;
     std::string err;
 };
@@ -158,7 +159,7 @@ int device_error(qa_ctx* ctx, int code, const char* which);
 // After a launch or device error the affected sequence restarts from position 0, like the
 // engine's "Errors ... reset all model ... state" (engine/INTERFACE.md error contract).
 int after_launch(qa_ctx* ctx, int seq, const char* what) {
-    ctx->last_fused_step = false;
+    ctx->last_fused_step = ctx->last_gather_wait = false;
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) return QA_OK;
     if (seq >= 0 && seq < (int)ctx->pos.size()) {
@@ -1460,6 +1461,7 @@ int qa_decode_step_gather(qa_ctx* ctx, int seq, int layer, int n_layers, int pos
                             landing, full, (size_t)n_layers * g.out_hq * D, ctx->error, ctx->stream);
     st = after_launch(ctx, -1, "gather_wait_copy");
     ctx->last_fused_step = chain && st == QA_OK;
+    ctx->last_gather_wait = true;
     return st;
 }
 
@@ -1567,6 +1569,13 @@ int check_tensor(qa_ctx* ctx, const void* p, const char* name) {
     return QA_OK;
 }
 
+// Whether a paged launch may start while the launch before it ends and wait for its end alone: not behind
+// the wait of a gather. The launch ends a chain of fused steps.
+bool may_overlap(qa_ctx* ctx) {
+    ctx->last_fused_step = false;
+    return !ctx->last_gather_wait;
+}
+
 int check_ints(qa_ctx* ctx, const void* p, const char* name) {
     if (!p || !aligned(p, 4)) return fail(ctx, QA_ERR_INVALID, "%s is null or not aligned", name);
     return QA_OK;
@@ -1612,7 +1621,7 @@ int qa_paged_append(qa_ctx* ctx, const qa_pages* pages, const int* table, int n_
     c.out[0] = q_out; c.out_floats[0] = q_out ? qn : 0;
     return run_call(ctx, -1, layer, n_layers, c, [&](int l0, int nl, const float* const* din, float* const* dout) {
         a.q_pre = din[0]; a.k_pre = din[1]; a.v_pre = din[2]; a.q_out = q_out ? dout[0] : nullptr;
-        a.layer0 = l0; a.n_layers = nl;
+        a.layer0 = l0; a.n_layers = nl; a.overlap = may_overlap(ctx);
         launch_paged_append(a, ctx->stream);
         return after_launch(ctx, -1, "paged_append");
     });
@@ -1652,8 +1661,7 @@ int qa_paged_attn(qa_ctx* ctx, const qa_pages* pages, const int* table, int tabl
     c.out[0] = out; c.out_floats[0] = qn;
     c.inputs_read_once = decode_inputs_read_once(n_layers, n, ctx->hkv);
     return run_call(ctx, -1, layer, n_layers, c, [&](int l0, int nl, const float* const* din, float* const* dout) {
-        a.q = din[0]; a.out = dout[0]; a.layer0 = l0; a.n_layers = nl;
-        ctx->last_fused_step = false;
+        a.q = din[0]; a.out = dout[0]; a.layer0 = l0; a.n_layers = nl; a.overlap = may_overlap(ctx);
         const cudaError_t e = launch_paged_attn(a, map, workspace, ctx->stream);
         if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, e, "paged_attn"); }
         return after_launch(ctx, -1, "paged_attn");
@@ -1679,7 +1687,7 @@ int qa_paged_evict(qa_ctx* ctx, const qa_pages* pages, const int* src_table, int
     a.src_table = src_table; a.src_cols = src_cols; a.dst_table = dst_table; a.dst_cols = dst_cols;
     a.lengths = lengths; a.new_lengths = new_lengths; a.n = n; a.keep = keep; a.recent = recent; a.kept = kept;
     a.error = ctx->error;
-    ctx->last_fused_step = false;
+    a.overlap = may_overlap(ctx);
     const cudaError_t e = launch_paged_evict(a, ctx->stream);
     if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, e, "paged_evict"); }
     return after_launch(ctx, -1, "paged_evict");

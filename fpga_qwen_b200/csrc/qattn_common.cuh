@@ -222,6 +222,7 @@ struct PagedAppendArgs {
     const float* norms; const float* cosines; const float* sines;
     float eps;
     int* error;
+    bool overlap;                             // the launch may start while the one before it ends (it waits for it)
 };
 void launch_paged_append(const PagedAppendArgs& a, cudaStream_t s);
 
@@ -236,6 +237,7 @@ struct PagedAttnArgs {
     void* shared;                             // [ranges][2] parts of units shared between ranges
     float* logits;                            // with add_weights: [16-row block][16][2]
     int* error;
+    bool overlap;
 };
 constexpr int MAX_PAGED_BATCH = 1024;
 size_t paged_attn_workspace(int n, int n_layers, int hkv, int max_rows, bool add_weights);
@@ -249,6 +251,7 @@ struct PagedEvictArgs {
     int n, keep, recent;
     int* kept;                                // [n][layers][hkv][keep]
     int* error;
+    bool overlap;
 };
 cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t s);
 

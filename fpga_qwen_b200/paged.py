@@ -147,8 +147,8 @@ class PagedSequences:
     def _check_inputs(self, n, layers, **tensors):
         heads = {"q": self.ctx.hq, "k": self.ctx.hkv, "v": self.ctx.hkv}
         for name, t in tensors.items():
-            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()):
-                raise QAttnError(QA_ERR_INVALID, f"{name} must be a contiguous float32 CUDA tensor")
+            if not (isinstance(t, torch.Tensor) and t.device == self.table.device and t.dtype == torch.float32 and t.is_contiguous()):
+                raise QAttnError(QA_ERR_INVALID, f"{name} must be a contiguous float32 tensor on {self.table.device}")
             if tuple(t.shape) != (layers, n, heads[name], 128):
                 raise QAttnError(QA_ERR_INVALID, f"{name} has shape {tuple(t.shape)}")
 
