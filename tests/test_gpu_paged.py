@@ -775,6 +775,66 @@ def test_evict_is_capturable_and_pairs_with_attention():
     assert not any(r[:, 2].any() for r in results[0][:9])
 
 
+def test_calls_in_a_row_equal_calls_one_by_one():
+    """Paged calls between slot calls, each reading what the one before wrote, queued without a wait and
+    with one after every call: the same bits. (Launches overlap; every kernel waits for the one before.)"""
+    L, rows = 2, 130
+    results = []
+    for wait in (False, True):
+        ctx = make(L, 8, context=512)
+        ctx.rope_positions(600)
+        c = Cache([rows, 40, 0], L, 8, seed=91, room=64)
+        lens, live = i32(c.lengths), i32([1, 1, 0])
+        pos, first = i32([300, 40, 0]), i32([0, 1, 2])
+        g = torch.Generator("cuda").manual_seed(17)
+        q, k, v = (torch.randn(L, 3, h, D, device="cuda", generator=g) for h in (16, 8, 8))
+        pq, pk, pv = (torch.randn(L, rows, h, D, device="cuda", generator=g) for h in (16, 8, 8))
+        qn, out, pqn, pout = (torch.zeros_like(t) for t in (q, q, pq, pq))
+        sq, sk, sv = (torch.zeros(L, 1, h, D, device="cuda") for h in (16, 8, 8))
+        sqn, sout = torch.zeros_like(sq), torch.zeros_like(sq)
+        size = ctx.paged_workspace(3, L, c.cols * c.page, True)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        kept = torch.zeros(3, L, 8, 60, dtype=torch.int32, device="cuda")
+        w = torch.randn(2048, 2048, device="cuda", generator=g).half()
+        y = torch.zeros(L, 3, 2048, device="cuda")
+        done = (lambda: ctx.sync()) if wait else (lambda: None)
+        seen = []
+        ctx.reset(0)
+        # a prompt into a slot, its rows into the pages of the first sequence
+        ctx.append(0, 0, L, 0, rows, pq.data_ptr(), pk.data_ptr(), pv.data_ptr(), pqn.data_ptr()); done()
+        ctx.attn_prefill(0, 0, L, 0, rows, pqn.data_ptr(), pout.data_ptr()); done()
+        ctx.commit(0, rows)
+        held = torch.arange(1, rows + 1, dtype=torch.int32, device="cuda")
+        at, seq0 = held - 1, torch.zeros_like(held)
+        ctx.paged_append(c.pages, c.table.data_ptr(), 3, c.cols, seq0.data_ptr(), held.data_ptr(), at.data_ptr(), rows, 0, L,
+                         pq.data_ptr(), pk.data_ptr(), pv.data_ptr(), pqn.data_ptr()); done()
+        for i in range(12):
+            lens.add_(live); done()
+            for layer in range(L):
+                ctx.paged_append(c.pages, c.table.data_ptr(), 3, c.cols, first.data_ptr(), lens.data_ptr(), pos.data_ptr(), 3, layer, 1,
+                                 q[layer].data_ptr(), k[layer].data_ptr(), v[layer].data_ptr(), qn[layer].data_ptr()); done()
+                ctx.paged_attn(c.pages, c.table.data_ptr(), c.cols, lens.data_ptr(), 3, layer, 1, qn[layer].data_ptr(),
+                               out[layer].data_ptr(), True, ws.data_ptr(), size); done()
+                # the next inputs come from this output: a projection, and a slot's decode step of its first row
+                ctx.project_gemm(w.data_ptr(), 2048, 2048, out[layer].data_ptr(), 3, y[layer].data_ptr()); done()
+            q.copy_(y.view(L, 3, 16, D)); done()
+            sq.copy_(out[:, :1]); sk.copy_(out[:, :1, :8]); sv.copy_(out[:, :1, 8:]); done()
+            ctx.decode_step(0, 0, L, rows + i, sq.data_ptr(), sk.data_ptr(), sv.data_ptr(), sqn.data_ptr(), sout.data_ptr()); done()
+            ctx.commit(0, 1)
+            # straight behind the step: attention of its queries, then an eviction
+            ctx.paged_attn(c.pages, c.table[:1].data_ptr(), c.cols, lens.data_ptr(), 1, 0, L, sqn.data_ptr(), sout.data_ptr(),
+                           True, ws.data_ptr(), size); done()
+            if i % 5 == 4:
+                ctx.paged_evict(c.pages, c.table.data_ptr(), c.cols, c.table.data_ptr(), c.cols, lens.data_ptr(), lens.data_ptr(), 3,
+                                60, 7, kept.data_ptr()); done()
+            pos.add_(live); done()
+            seen += [out.clone(), sout.clone(), kept.clone(), lens.clone()]
+        ctx.sync()
+        results.append(seen + [pout, c.kv.clone(), c.w.clone()])
+    for x, y in zip(*results):
+        assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+
+
 # ---- host buffers, refusals, bad tables ----------------------------------------------------------
 def test_host_buffer_context():
     L, hkv, n = 3, 8, 5
