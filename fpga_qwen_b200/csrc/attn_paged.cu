@@ -85,6 +85,12 @@ struct Part {
     long long g;                              // its first block in the call
     float m[GROUP], l[GROUP];
 };
+// A unit that a CTA merged: all of its blocks (cnt), or not (0).
+struct Whole {
+    int unit, cnt;
+    long long g;
+    float m[GROUP], l[GROUP];
+};
 // The joining launch's view of a range's part of a shared unit.
 struct __align__(16) Shared {
     int nrec, first, first_slot, unit;        // records of the unit (0: no such part), their first range and its slot
@@ -93,9 +99,9 @@ struct __align__(16) Shared {
 };
 // A CTA's part of its cluster's unit.
 struct Joint {
-    int cnt;                                  // blocks, 0: none
-    float m[GROUP], l[GROUP];
     float o[GROUP * D];
+    float m[GROUP], l[GROUP];
+    int cnt;                                  // blocks, 0: none
 };
 __device__ __forceinline__ Shared* shared_of(const PagedAttnArgs& a) { return static_cast<Shared*>(a.shared); }
 
@@ -207,7 +213,8 @@ __global__ void __launch_bounds__(W * 32, 1) attn_paged_split_kernel(const Paged
     __shared__ int warp_sum[WARPS];
     __shared__ Part parts[W][2];                             // [0]: of the warp's first unit, [1]: of its last
     __shared__ __align__(16) float s_part[W][2][GROUP * D];
-    __shared__ Joint joint;
+    __shared__ Whole wholes[WEIGHTS ? W * 2 : 1];            // of the merged units, by turn
+    __shared__ __align__(16) Joint joint;
     __shared__ int abort_flag, never_abort;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
     const int g8 = lane >> 2, j4 = lane & 3, head = j4 & 1;  // tile row or column, and the column pair's head
@@ -247,6 +254,7 @@ __global__ void __launch_bounds__(W * 32, 1) attn_paged_split_kernel(const Paged
             if (tid < 2) shared_of(a)[c * 2 + tid].nrec = 0;
             return;
         }
+        if (tid < 2) shared_of(a)[c * 2 + tid].nrec = 0;     // until the merge finds a shared unit
         c_begin = sp.begin(c);
         c_blocks = (int)(sp.begin(c + 1) - c_begin);
     }
@@ -472,23 +480,28 @@ __global__ void __launch_bounds__(W * 32, 1) attn_paged_split_kernel(const Paged
     __syncthreads();
 
     // ---- merge the warps' parts: those of one unit are neighbours in the order of the blocks ----
-    // every warp holds all parts, two lanes each: lane is part lane % 16 and head lane / 16
-    static_assert(W * 2 <= 16 && GROUP * D % T == 0, "two heads of all parts within a warp; whole rounds of columns");
+    // A single unit by all threads, a column or two each; several by a warp each (64 ragged rows 95.5 -> 94.2 us,
+    // 33 of up to 512 17.9 -> 16.3 us against one after the other; a single unit is 0.3 us faster by all).
+    // Every warp holds all parts, two lanes each: lane is part lane % 16 and head lane / 16.
+    static_assert(W * 2 <= 16 && GROUP * D % T == 0, "two heads of all parts fit a warp; whole rounds of columns");
     const int part = lane & 15, part_head = lane >> 4;
     Part p{};
     p.unit = -1;
     if (part < W * 2) p = parts[part >> 1][part & 1];
     const float p_m = part_head ? p.m[1] : p.m[0], p_l = part_head ? p.l[1] : p.l[0];
-    unsigned left = __ballot_sync(0xffffffffu, p.unit >= 0) & 0xffff;
-    unsigned have = 0;                                       // records of this range
-    while (left) {
+    const unsigned all = __ballot_sync(0xffffffffu, p.unit >= 0) & 0xffff;
+    bool single = true;
+    int turn = 0;                                            // units so far
+    for (unsigned left = all; left; ++turn) {
         const int first = __ffs(left) - 1;
-        const int unit = __shfl_sync(0xffffffffu, p.unit, first), blk0 = __shfl_sync(0xffffffffu, p.blk0, first);
-        const int nblk = __shfl_sync(0xffffffffu, p.nblk, first);
-        const long long g = __shfl_sync(0xffffffffu, p.g, first);
+        const int unit = __shfl_sync(0xffffffffu, p.unit, first);
         const bool mine = p.unit == unit;
         const unsigned group = __ballot_sync(0xffffffffu, mine) & 0xffff;
         left &= ~group;
+        single = group == all;
+        if (!single && turn % W != warp) continue;
+        const int blk0 = __shfl_sync(0xffffffffu, p.blk0, first), nblk = __shfl_sync(0xffffffffu, p.nblk, first);
+        const long long g = __shfl_sync(0xffffffffu, p.g, first);
         const int cnt = __reduce_add_sync(0xffffffffu, mine && part_head == 0 ? p.cnt : 0);
         float top = mine ? p_m : -INFINITY;
         #pragma unroll
@@ -499,56 +512,88 @@ __global__ void __launch_bounds__(W * 32, 1) attn_paged_split_kernel(const Paged
         for (int x = 8; x >= 1; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
         const float M[GROUP] = {__shfl_sync(0xffffffffu, top, 0), __shfl_sync(0xffffffffu, top, 16)};
         const float L[GROUP] = {__shfl_sync(0xffffffffu, sum, 0), __shfl_sync(0xffffffffu, sum, 16)};
-        constexpr int COLS = GROUP * D / T;                  // of a thread, T apart
-        float o[COLS];
-        #pragma unroll
-        for (int x = 0; x < COLS; ++x) {
-            const int col = x * T + tid;
-            o[x] = 0.f;
+        const int slot = g != c_begin;
+        float* rec = a.records + ((size_t)c * 2 + slot) * PARTIAL_FLOATS;
+        if (single) {
+            constexpr int COLS = GROUP * D / T;              // of a thread, T apart
+            float o[COLS];
             #pragma unroll
-            for (int k = 0; k < W * 2; ++k) {
-                const float fk = __shfl_sync(0xffffffffu, f, k + (col >= D ? 16 : 0));   // (a warp's columns are of one head)
-                if (group >> k & 1) o[x] += fk * s_part[k >> 1][k & 1][col];
+            for (int x = 0; x < COLS; ++x) {
+                const int col = x * T + tid;
+                o[x] = 0.f;
+                #pragma unroll
+                for (int k = 0; k < W * 2; ++k) {
+                    const float fk = __shfl_sync(0xffffffffu, f, k + (col >= D ? 16 : 0));   // (a warp's columns are of one head)
+                    if (group >> k & 1) o[x] += fk * s_part[k >> 1][k & 1][col];
+                }
+            }
+            if (cnt == nblk) {
+                #pragma unroll
+                for (int x = 0; x < COLS; ++x)
+                    a.out[(size_t)unit * GROUP * D + x * T + tid] = o[x] / (x * T + tid >= D ? L[1] : L[0]);
+                if (WEIGHTS) {
+                    const int lb = unit / hkv, row_l = lb / a.n, row_b = lb - row_l * a.n, row_kh = unit - lb * hkv;
+                    add_weights(a, row_l, row_b, row_kh, row_length(a, row_b), 0, cnt, g, M, L, tid, T);
+                }
+            } else if (alone) {
+                #pragma unroll
+                for (int x = 0; x < COLS; ++x) joint.o[x * T + tid] = o[x];
+                if (tid < GROUP) { joint.m[tid] = tid ? M[1] : M[0]; joint.l[tid] = tid ? L[1] : L[0]; }
+                if (tid == 0) joint.cnt = cnt;
+            } else {
+                #pragma unroll
+                for (int x = 0; x < COLS; ++x) rec[4 + x * T + tid] = o[x];
+            }
+        } else if (W == WARPS) {
+            float4 o[GROUP];                                 // channels 4 lane to 4 lane + 3 of both heads
+            #pragma unroll
+            for (int k = 0; k < GROUP; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (unsigned parts_left = group; parts_left; parts_left &= parts_left - 1) {
+                const int i = __ffs(parts_left) - 1;
+                #pragma unroll
+                for (int k = 0; k < GROUP; ++k) {
+                    const float fk = __shfl_sync(0xffffffffu, f, i + 16 * k);
+                    const float4 x = reinterpret_cast<const float4*>(s_part[i >> 1][i & 1] + k * D)[lane];
+                    o[k].x += fk * x.x; o[k].y += fk * x.y; o[k].z += fk * x.z; o[k].w += fk * x.w;
+                }
+            }
+            const bool whole = cnt == nblk;
+            if (WEIGHTS && lane == 0) {
+                Whole& w = wholes[turn];
+                w.unit = unit; w.cnt = whole ? cnt : 0; w.g = g;
+                w.m[0] = M[0]; w.m[1] = M[1]; w.l[0] = L[0]; w.l[1] = L[1];
+            }
+            #pragma unroll
+            for (int k = 0; k < GROUP; ++k) {
+                if (whole)
+                    reinterpret_cast<float4*>(a.out + ((size_t)unit * GROUP + k) * D)[lane] =
+                        make_float4(o[k].x / L[k], o[k].y / L[k], o[k].z / L[k], o[k].w / L[k]);
+                else
+                    reinterpret_cast<float4*>(rec + 4 + k * D)[lane] = o[k];
             }
         }
-        if (cnt == nblk) {
-            #pragma unroll
-            for (int x = 0; x < COLS; ++x)
-                a.out[(size_t)unit * GROUP * D + x * T + tid] = o[x] / (x * T + tid >= D ? L[1] : L[0]);
-            // the weights of a short unit by one warp, while the others go on to the next unit
-            const bool by_all = cnt > 4 * W;
-            if (WEIGHTS && (by_all || warp == (first >> 1))) {
-                const int lb = unit / hkv, row_l = lb / a.n, row_b = lb - row_l * a.n, row_kh = unit - lb * hkv;
-                add_weights(a, row_l, row_b, row_kh, row_length(a, row_b), 0, cnt, g, M, L, by_all ? tid : lane, by_all ? T : 32);
-            }
-        } else if (alone) {
-            #pragma unroll
-            for (int x = 0; x < COLS; ++x) joint.o[x * T + tid] = o[x];
-            if (tid < GROUP) { joint.m[tid] = tid ? M[1] : M[0]; joint.l[tid] = tid ? L[1] : L[0]; }
-            if (tid == 0) joint.cnt = cnt;
-        } else {
-            const int slot = g != c_begin;
-            float* rec = a.records + ((size_t)c * 2 + slot) * PARTIAL_FLOATS;
-            if (tid < GROUP) { rec[tid] = M[tid]; rec[GROUP + tid] = L[tid]; }
-            #pragma unroll
-            for (int x = 0; x < COLS; ++x) rec[4 + x * T + tid] = o[x];
-            if (tid == slot * 32) {
-                const long long off = g - blk0;
-                Shared s;
-                s.first = sp.range_of(off);
-                s.nrec = sp.range_of(off + nblk - 1) - s.first + 1;
-                s.first_slot = off != sp.begin(s.first);
-                s.unit = unit; s.blk0 = blk0; s.cnt = cnt; s.g = g;
-                shared_of(a)[c * 2 + slot] = s;
-            }
-            have |= 1u << slot;
+        if (!alone && cnt != nblk && lane == 0 && (!single || warp == 0)) {
+            *reinterpret_cast<float4*>(rec) = make_float4(M[0], M[1], L[0], L[1]);
+            const long long off = g - blk0;
+            Shared s;
+            s.first = sp.range_of(off);
+            s.nrec = sp.range_of(off + nblk - 1) - s.first + 1;
+            s.first_slot = off != sp.begin(s.first);
+            s.unit = unit; s.blk0 = blk0; s.cnt = cnt; s.g = g;
+            shared_of(a)[c * 2 + slot] = s;
         }
     }
-    if (!alone) {
-        if (tid < 2 && !(have >> tid & 1)) shared_of(a)[c * 2 + tid].nrec = 0;
-        return;
+    if (WEIGHTS && !single) {
+        __syncthreads();
+        for (int e = 0; e < turn; ++e) {
+            const Whole w = wholes[e];
+            const bool by_all = w.cnt > 4 * W;               // those of a short unit by one warp
+            if (w.cnt == 0 || !(by_all || warp == e % W)) continue;
+            const int lb = w.unit / hkv, row_l = lb / a.n, row_b = lb - row_l * a.n, row_kh = w.unit - lb * hkv;
+            add_weights(a, row_l, row_b, row_kh, row_length(a, row_b), 0, w.cnt, w.g, w.m, w.l, by_all ? tid : lane, by_all ? T : 32);
+        }
     }
-    if (alone == 1) return;
+    if (alone <= 1) return;
     // ---- join the cluster's parts (none where one CTA held the whole unit) ----
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
