@@ -261,7 +261,8 @@ typedef struct qa_pages {
     uint16_t* kv;        /* [n_pages][n_layers][K|V][hkv_local][page_rows][128] FP16, 16-byte aligned */
     float* weights;      /* [n_pages][n_layers][hkv_local][page_rows] FP32 accumulated attention
                             weights, 16-byte aligned; NULL where no call uses them */
-    int n_pages;
+    int n_pages;         /* qa_paged_attn: n_pages * n_layers * 2 * hkv_local * page_rows < 2^31
+                            (QA_ERR_UNSUPPORTED) */
     int page_rows;       /* 16, 32, 64, 128, 256 or 512 */
 } qa_pages;
 
