@@ -22,13 +22,17 @@
 //     round trips, for no more bytes.)
 //
 // Numerics: FP16 rows are exact operands. A query (scaled by a power of two so that its largest
-// channel lies in [2^13, 2^14)) and a weight (exp2 of the distance to the maximum, plus 14) are
-// each the sum of two FP16 halves: 22 bits, or 2^-38 of the largest, whichever is coarser; sums are
-// FP32, and long sums are made by FADD: the tensor core's own accumulation truncates, which over the
-// hundred blocks of a long history costs a few 2^-20 (2.0e-6 off in 2-norm against 64 bits at
-// 131071 rows), so it takes no more than two steps of a chain. The high half is rounded towards zero and
-// neither half of a nonzero value is zero, so both have its sign and an infinite key or value gives
-// what the formula gives.
+// channel lies in [2^13, 2^14)) and a weight (exp2 of the distance to its block's maximum, plus 14) are
+// each the sum of two FP16 halves: off by 2^-22 of the value, or by 2^-36 of the largest channel and
+// 2^-37 of the block's largest weight, whichever is coarser. Sums are FP32, and long sums are made by
+// FMA, with the block's factor (exp2 of the distance of its maximum to the running one): the tensor core's own
+// accumulation truncates, which over the hundred blocks of a long history costs a few 2^-20 (2.0e-6 off in
+// 2-norm against 64 bits at 131071 rows), so it takes no more than two steps of a chain. The high half is
+// rounded towards zero and neither half of a nonzero value is zero, so both have its sign and an infinite key or
+// value gives what the formula gives. That adds 2^-37 of the largest to a weight far below it, all of one sign, which is
+// why weights are relative to their own block: against the running maximum one heavy row did so to every row after
+// it (131071 rows 25 to 80 nats below one, their values 10^5 times as large: outputs off by up to 0.7%, now by
+// 1.5e-5, the part of the heavy row's own block; times of whole calls are the same within 1%).
 //
 // A unit that several warps of a CTA share is merged through shared memory at the CTA's end; a
 // unit that several CTAs share leaves one record (max, sum, 2 x 128 partial output) per CTA, and a
@@ -418,8 +422,10 @@ __global__ void __launch_bounds__(W * 32, 1) attn_paged_split_kernel(const Paged
                             #pragma unroll
                             for (int e = 0; e < 4; ++e) acc[i][e] *= scale;
                     }
-                    const float p0 = g8 < rows ? exp2_from(s0, m) : 0.f, p1 = g8 + 8 < rows ? exp2_from(s1, m) : 0.f;
-                    l += p0 + p1;
+                    // weights of the block's own maximum, whose halves therefore hold them, and the block's factor
+                    const float p0 = g8 < rows ? exp2_from(s0, mb) : 0.f, p1 = g8 + 8 < rows ? exp2_from(s1, mb) : 0.f;
+                    const float factor = exp2_from(mb, m);
+                    l += factor * (p0 + p1);
                     // this lane's operand: rows 2 j4 + {0, 1, 8, 9} of column g8 (head (g8 / 2) % 2, half g8 % 2)
                     const uint32_t h0 = split_half(p0), h1 = split_half(p1);
                     const int from = 8 * j4 + (g8 >> 1 & 1);
@@ -435,7 +441,7 @@ __global__ void __launch_bounds__(W * 32, 1) attn_paged_split_kernel(const Paged
                         float pv[4];
                         mma16816_new(pv, vf, b0, b1);
                         #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][e] += pv[e];
+                        for (int e = 0; e < 4; ++e) acc[i][e] += factor * pv[e];
                     }
                 }
                 __syncwarp();                                // the stage is read by all lanes

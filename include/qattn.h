@@ -297,8 +297,11 @@ int qa_paged_workspace(const qa_ctx* ctx, int n, int n_layers, int max_rows, int
 
 /* Attention of one query row per sequence over its pages, split over the cache's length and
  * joined (flash-decoding): row b attends to cache rows [0, lengths[b]) of table row b, softmax(q.k /
- * sqrt(128)) . V in FP32, as qa_attn_decode_batch does over slots. lengths (device, n ints) count
- * the new row once it is appended; a row of length 0 (padding) gives zeros. Rows may share pages.
+ * sqrt(128)) . V, as qa_attn_decode_batch does over slots. Sums are FP32; queries and softmax
+ * weights enter the products as two FP16 halves, off by 2^-22 of the value, or by 2^-36 of the row's largest
+ * query channel and 2^-37 of the largest weight among the 16 cache rows of a block, whichever is
+ * coarser. lengths (device, n ints) count the new row once it is appended; a row of length 0 (padding)
+ * gives zeros. Rows may share pages.
  * q, out: [n_layers][n][hq_local][128], 16-byte aligned; 1 <= n <= QA_MAX_PAGED_BATCH.
  * add_weights != 0 also adds, for every cache row and KV head, the softmax weights of the head's
  * query heads to pages->weights (one FP32 addition per call and row, so the results are
