@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(W * 32, 1) attn_paged_split_kernel(const Paged
         const int i = c / alone, rank = c - i * alone;       // the CTA's unit, and its place in the cluster
         only = paged_unit_alone(i, a.n, hkv, ((a.cols << a.kv.shift) + BLK - 1) / BLK);
         const int given = a.lengths[only.b], len = paged_length(given, a.cols, a.kv.shift);
-        if (given != len && tid == 0) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
+        if (given != len && tid == 0) atomicCAS(a.error + ERR_DATA, 0, PAGED_BAD_LENGTH);
         only.nblk = (len + BLK - 1) / BLK;
         if (len == 0) {                                      // (for the whole cluster)
             for (int col = tid; rank == 0 && col < GROUP * D; col += T) a.out[(size_t)i * GROUP * D + col] = 0.f;
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(W * 32, 1) attn_paged_split_kernel(const Paged
             valid = ok ? valid | 1u << stage : valid & ~(1u << stage);
             if (lane == 0) {
                 if (ok) mbar_arrive_expect_tx(&my_full[stage], STAGE);
-                else { mbar_arrive(&my_full[stage]); atomicCAS(a.error, 0, PAGED_BAD_PAGE); }
+                else { mbar_arrive(&my_full[stage]); atomicCAS(a.error + ERR_DATA, 0, PAGED_BAD_PAGE); }
             }
             __syncwarp();
             if (ok && lane < 4) {                            // lane: K or V, channel half
@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, 5) attn_paged_join_kernel(const 
     const int part = blockIdx.y;
     const int row_floats = GROUP * a.kv.hkv * D;
     for (int b = tid; b < a.n && blockIdx.x + part == 0; b += JOIN_THREADS)
-        if (a.lengths[b] != row_length(a, b)) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
+        if (a.lengths[b] != row_length(a, b)) atomicCAS(a.error + ERR_DATA, 0, PAGED_BAD_LENGTH);
     for (int i = blockIdx.x; part == 0 && i < a.n_layers * a.n; i += gridDim.x)
         if (row_length(a, i % a.n) == 0)
             for (int j = tid * 4; j < row_floats; j += JOIN_THREADS * 4)

@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const PagedEv
         for (int i = tid; i < dst_used; i += SEL_THREADS) s_dst[i] = dst[i];
         dst = s_dst;
     }
-    if (tid == 0 && rank == 0 && a.lengths[b] != L) atomicCAS(a.error, 0, PAGED_BAD_LENGTH);
+    if (tid == 0 && rank == 0 && a.lengths[b] != L) atomicCAS(a.error + ERR_DATA, 0, PAGED_BAD_LENGTH);
     #pragma unroll 1
     for (int i0 = tid; i0 < rows; i0 += SEL_THREADS * BATCH) {
         // all page ids of a batch, then all its weights, in flight at once
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const PagedEv
             bad |= !ok;
             w[k] = ok && i < rows ? *a.kv.weight(page[k], layer, h, (row0 + i) & mask) : 0.f;
         }
-        if (bad) atomicCAS(a.error, 0, PAGED_BAD_PAGE);
+        if (bad) atomicCAS(a.error + ERR_DATA, 0, PAGED_BAD_PAGE);
         #pragma unroll
         for (int k = 0; k < BATCH; ++k)
             if (i0 + k * SEL_THREADS < rows) s_w[i0 + k * SEL_THREADS] = w[k];
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const PagedEv
             kept[j] = row0 + i;
             const int page = dst[j >> a.kv.shift];
             if (a.kv.has(page)) *a.kv.weight(page, layer, h, j & mask) = s_w[i];
-            else atomicCAS(a.error, 0, PAGED_BAD_PAGE);
+            else atomicCAS(a.error + ERR_DATA, 0, PAGED_BAD_PAGE);
         }
         above += __popc(up);
         ties += __popc(tie);

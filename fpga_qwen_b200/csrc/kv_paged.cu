@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(32) kv_paged_append_kernel(const PagedAppendAr
     int code = 0, page = -1;
     if (lane < ntok)
         page = paged_place(len, seq, pos, a.n_seqs, a.cols, a.kv.shift, a.rope_rows, a.kv.n_pages, a.table, &code);
-    if (code) atomicCAS(a.error, 0, code);
+    if (code) atomicCAS(a.error + ERR_DATA, 0, code);
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
     float inv = 0.f;                                      // of row `lane`

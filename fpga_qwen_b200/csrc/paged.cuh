@@ -14,8 +14,8 @@
 
 namespace qattn {
 
-// Codes left in the error block for page tables, lengths and positions read on the device
-// (reported as QA_ERR_INVALID; every other code is an expired wait).
+// Codes left in the error block's ERR_DATA word for page tables, lengths and positions read on the device
+// (reported as QA_ERR_INVALID).
 constexpr int PAGED_BAD_LENGTH = 61, PAGED_BAD_PAGE = 62, PAGED_BAD_POSITION = 63, PAGED_BAD_SEQ = 64;
 
 // A length as the kernels use it: one outside its table (cols pages of 1 << shift rows) is 0.

@@ -148,7 +148,8 @@ int cuda_fail(qa_ctx* c, cudaError_t e, const char* what) {
     return fail(c, e == cudaErrorMemoryAllocation ? QA_ERR_OOM : QA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-int device_error(qa_ctx* ctx, int code, const char* which);
+int wait_error(qa_ctx* ctx, int code, const char* which);
+int data_error(qa_ctx* ctx, int code);
 
 #define QA_CUDA(call)                                                  \
     do {                                                               \
@@ -242,6 +243,7 @@ struct IoCall {
     // PCIe; false where many CTAs read the same rows (a decode whose units are split many ways),
     // which then goes through the staging copies (measured faster for one-layer decode calls)
     bool inputs_read_once = true;
+    bool paged = false;            // reports data errors of paged calls
 };
 
 // launch(l0, nl, din, dout) enqueues the work of layers [l0, l0 + nl) on device pointers and
@@ -263,7 +265,12 @@ int io_host_call(qa_ctx* ctx, int seq, int layer, int n_layers, const IoCall& c,
                 ctx->pos[seq] = 0;
                 std::fill(ctx->appended[seq].begin(), ctx->appended[seq].end(), 0);
             }
-            return device_error(ctx, code, "the call's results are invalid");
+            return wait_error(ctx, code, "the call's results are invalid");
+        }
+        if (const int code = c.paged ? h_err[ERR_DATA] : 0) {
+            QA_CUDA(cudaMemsetAsync(ctx->error + ERR_DATA, 0, sizeof(int), ctx->stream));
+            QA_CUDA(cudaStreamSynchronize(ctx->stream));
+            return data_error(ctx, code);
         }
         return QA_OK;
     };
@@ -408,26 +415,30 @@ int make_rope_tables(qa_ctx* ctx, int n) {
     return QA_OK;
 }
 
-// The status and message of a code that the device left in the error block.
-int device_error(qa_ctx* ctx, int code, const char* which) {
+// The status and message of a code that the device left in the error block: ERR_CODE, ERR_DATA.
+int wait_error(qa_ctx* ctx, int code, const char* which) {
+    return fail(ctx, QA_ERR_TIMEOUT, "a device-side wait expired (code %d); %s", code, which);
+}
+int data_error(qa_ctx* ctx, int code) {
     switch (code) {
         case PAGED_BAD_LENGTH: return fail(ctx, QA_ERR_INVALID, "a paged call met a length outside its table (code %d)", code);
         case PAGED_BAD_PAGE: return fail(ctx, QA_ERR_INVALID, "a paged call met a page id outside the pool (code %d)", code);
         case PAGED_BAD_POSITION: return fail(ctx, QA_ERR_INVALID, "a paged append met a position outside the RoPE tables (code %d)", code);
         case PAGED_BAD_SEQ: return fail(ctx, QA_ERR_INVALID, "a paged append met a sequence outside the table (code %d)", code);
-        default: return fail(ctx, QA_ERR_TIMEOUT, "a device-side wait expired (code %d); %s", code, which);
+        default: return fail(ctx, QA_ERR_INVALID, "a paged call met bad data (code %d)", code);
     }
 }
 
-// Reads and clears the device error flag of the bounded waits and the paged calls.
+// Reads and clears the device error flag of the bounded waits or, where no wait expired, that of the paged calls.
 int check_device_error(qa_ctx* ctx) {
-    int code = 0;
-    QA_CUDA(cudaMemcpyAsync(&code, ctx->error, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
+    int words[ERR_DATA + 1] = {};
+    QA_CUDA(cudaMemcpyAsync(words, ctx->error, sizeof words, cudaMemcpyDeviceToHost, ctx->stream));
     QA_CUDA(cudaStreamSynchronize(ctx->stream));
-    if (code) {
-        QA_CUDA(cudaMemsetAsync(ctx->error, 0, sizeof(int), ctx->stream));
-        return device_error(ctx, code, "results of the last calls are invalid");
-    }
+    for (const int word : {ERR_CODE, ERR_DATA})
+        if (words[word]) {
+            QA_CUDA(cudaMemsetAsync(ctx->error + word, 0, sizeof(int), ctx->stream));
+            return word == ERR_CODE ? wait_error(ctx, words[word], "results of the last calls are invalid") : data_error(ctx, words[word]);
+        }
     return QA_OK;
 }
 
@@ -1126,7 +1137,7 @@ int project_call(qa_ctx* ctx, int n_mats, const uint16_t* const* w, const int* r
     if (const int code = h_err[ERR_CODE]) {
         QA_CUDA(cudaMemsetAsync(ctx->error + ERR_CODE, 0, sizeof(int), ctx->stream));
         QA_CUDA(cudaStreamSynchronize(ctx->stream));
-        return device_error(ctx, code, "results of the last calls are invalid");
+        return wait_error(ctx, code, "results of the last calls are invalid");
     }
     return QA_OK;
 }
@@ -1617,6 +1628,7 @@ int qa_paged_append(qa_ctx* ctx, const qa_pages* pages, const int* table, int n_
     a.norms = ctx->norms; a.cosines = ctx->cosines; a.sines = ctx->sines; a.eps = ctx->cfg.norm_eps; a.error = ctx->error;
     const size_t qn = (size_t)n * ctx->hq * D, kn = (size_t)n * ctx->hkv * D;
     IoCall c;
+    c.paged = true;
     c.in[0] = q_pre; c.in[1] = k_pre; c.in[2] = v; c.in_floats[0] = qn; c.in_floats[1] = kn; c.in_floats[2] = kn;
     c.out[0] = q_out; c.out_floats[0] = q_out ? qn : 0;
     return run_call(ctx, -1, layer, n_layers, c, [&](int l0, int nl, const float* const* din, float* const* dout) {
@@ -1657,6 +1669,7 @@ int qa_paged_attn(qa_ctx* ctx, const qa_pages* pages, const int* table, int tabl
     if ((st = make_pages_map(ctx, a.kv, &map))) return st;
     const size_t qn = (size_t)n * ctx->hq * D;
     IoCall c;
+    c.paged = true;
     c.in[0] = q; c.in_floats[0] = qn;
     c.out[0] = out; c.out_floats[0] = qn;
     c.inputs_read_once = decode_inputs_read_once(n_layers, n, ctx->hkv);

@@ -67,7 +67,10 @@ constexpr int MAX_RANKS = 8;
 //                     by qa_sync and by every host-buffer call
 //   word ERR_WAIT_US  limit of the waits on other GPUs' flags, in microseconds (0 = 2 s)
 //   word ERR_NEVER    a flag word that nothing ever sets (qa_selftest_timeout waits on it)
-constexpr int ERR_CODE = 0, ERR_WAIT_US = 1, ERR_NEVER = 2;
+//   word ERR_DATA     first PAGED_BAD_* code of a paged call; read and cleared by qa_sync and by the
+//                     host-buffer calls on pages. Apart from ERR_CODE, so that it neither fails a call
+//                     on slots (which resets its sequence) nor hides an expired wait.
+constexpr int ERR_CODE = 0, ERR_WAIT_US = 1, ERR_NEVER = 2, ERR_DATA = 3;
 constexpr size_t ERR_BLOCK_BYTES = 256;
 __device__ __forceinline__ unsigned long long peer_wait_limit_ns(const int* error) {
     const unsigned us = *reinterpret_cast<const volatile unsigned*>(error + ERR_WAIT_US);

@@ -255,8 +255,9 @@ int qa_project_group_gemm(qa_ctx* ctx, int n_mats, const uint16_t* const* w, con
  * block; cache row t of a sequence is row t % page_rows of page table[t / page_rows].
  * Page ids, lengths and positions are read on the device: one outside its range is skipped
  * (nothing is read or written through it), the results of its sequence are undefined, and the
- * next qa_sync or host-buffer call returns QA_ERR_INVALID. Table entries past a sequence's
- * length are not read. */
+ * next qa_sync, or host-buffer call of qa_paged_append or qa_paged_attn, returns QA_ERR_INVALID
+ * (after QA_ERR_TIMEOUT, if a wait expired too). Calls on slots neither report it nor are touched
+ * by it. Table entries past a sequence's length are not read. */
 typedef struct qa_pages {
     uint16_t* kv;        /* [n_pages][n_layers][K|V][hkv_local][page_rows][128] FP16, 16-byte aligned */
     float* weights;      /* [n_pages][n_layers][hkv_local][page_rows] FP32 accumulated attention
