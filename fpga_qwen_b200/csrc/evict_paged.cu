@@ -297,7 +297,9 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const PagedEvi
 cudaError_t launch(void (*kernel)(PagedEvictArgs), dim3 grid, int threads, size_t smem, int cluster, bool overlap,
                    const PagedEvictArgs& a, cudaStream_t s) {
     cudaError_t e = cudaSuccess;
-    if (smem > 32 << 10) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // (the kernel's own most, whatever this call takes: the attribute is the kernel's, and another host thread may be
+    // between its own two calls)
+    if (smem > 32 << 10) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SLICE * (int)sizeof(float));
     if (e != cudaSuccess) return e;
     if (cluster > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
