@@ -84,6 +84,41 @@ class PageTable:
         self.rows[seq] = rows
 
 
+class StepOrder:
+    """Which layers of the step under way have their new rows. From begin_step, which counts the rows, to the append of
+    the last layer they are not all written: an eviction would take whatever their page held before, and another
+    begin_step would leave it behind for attention to read."""
+
+    def __init__(self, layers: int):
+        self.layers, self.unwritten, self.seqs, self.replays = layers, set(), set(), False
+
+    def begin(self, seqs):
+        self.seqs = set(seqs)
+        self.unwritten = set() if self.replays else set(range(self.layers))
+
+    def wrote(self, layer: int, n: int):
+        self.unwritten -= set(range(layer, layer + n))
+
+    def captured(self):
+        """An append was captured and not run: steps are made by replays from now on, which nothing here sees."""
+        self.replays = True
+        self.unwritten = set()
+
+    def close(self, seq: int):
+        self.seqs.discard(seq)
+        if not self.seqs:
+            self.unwritten = set()
+
+    def check_complete(self, what: str):
+        if self.unwritten:
+            raise QAttnError(QA_ERR_STATE, f"{what} before the step's rows are appended (layers {sorted(self.unwritten)})")
+
+    def check_written(self, layer: int, n: int):
+        missing = sorted(self.unwritten & set(range(layer, layer + n)))
+        if missing:
+            raise QAttnError(QA_ERR_STATE, f"attend before the step's rows of layers {missing} are appended")
+
+
 class PagedSequences:
     """Up to max_seqs sequences of a context over a pool of n_pages pages.
 
@@ -94,6 +129,11 @@ class PagedSequences:
     which go on past the cached rows once rows are evicted; ``step_layers`` is the most layers of one
     ``attend`` call (it sizes the workspace, which is made once, so that captured steps stay valid).
     One caller, and one stream, at a time, as for the context.
+
+    A step's rows count from ``begin_step`` on, so until ``append`` has written them in every layer ``evict``, another
+    ``begin_step`` and ``attend`` of a layer without them are refused (``QA_ERR_STATE``; closing the step's
+    sequences ends it). Once an ``append`` has been captured into a graph the replays, which nothing here sees,
+    are taken to follow their ``begin_step`` at once: that order is then the caller's to keep.
     """
 
     def __init__(self, ctx: Context, n_pages: int, page_rows: int = 16, max_seqs: int = 1, max_rows: int = 4096,
@@ -104,6 +144,7 @@ class PagedSequences:
         self.ctx, self.slot, self.layers = ctx, slot, ctx.config.n_layers
         self.max_position = max_position or max(max_rows, ctx.config.context)
         self.step_layers = self.layers if step_layers is None else step_layers
+        self.step = StepOrder(self.layers)
         ctx.rope_positions(self.max_position)
         dev = torch.device("cuda", ctx.config.device)
         self.kv = torch.zeros(n_pages, self.layers, 2, ctx.hkv, page_rows, 128, dtype=torch.float16, device=dev)
@@ -121,6 +162,7 @@ class PagedSequences:
 
     def close(self, seq: int):
         self.host.close(seq)
+        self.step.close(seq)
         self.lengths[seq] = 0
 
     def rows(self, seq: int) -> int:
@@ -198,7 +240,9 @@ class PagedSequences:
         live = self.host.live()
         if not live:
             raise QAttnError(QA_ERR_STATE, "no open sequence")
+        self.step.check_complete("begin_step")
         self._grow({seq: 1 for seq in live})
+        self.step.begin(live)
         held = [self.host.rows[seq] for seq in range(len(self.host.pages))]
         self.lengths.copy_(self._int32(held))
         self.positions.copy_(self._int32([max(p - 1, 0) for p in self.host.position]))
@@ -213,12 +257,18 @@ class PagedSequences:
         self.ctx.paged_append(self.pages, self.table.data_ptr(), n, self.host.cols, 0, self.lengths.data_ptr(),
                               self.positions.data_ptr(), n, layer, layers, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                               qn.data_ptr())
+        if not self.step.replays:
+            with torch.cuda.device(self.table.device):
+                if torch.cuda.is_current_stream_capturing():
+                    self.step.captured()
+        self.step.wrote(layer, layers)
         return qn
 
     def attend(self, qn, layer: int = 0, add_weights: bool = True, out=None):
         """Attention of the rows just appended; adds their weights for a later eviction."""
         layers, n = (qn.shape[0], self.table.shape[0]) if isinstance(qn, torch.Tensor) and qn.dim() else (0, 0)
         self._check_inputs(n, layers, q=qn)
+        self.step.check_written(layer, layers)
         out = torch.empty_like(qn) if out is None else out
         self._check_inputs(n, layers, q=out)
         self._stream()
@@ -233,6 +283,7 @@ class PagedSequences:
         n = self.table.shape[0]
         if keep < 1 or not 0 <= recent <= keep:
             raise QAttnError(QA_ERR_INVALID, f"keep {keep}, recent {recent}")
+        self.step.check_complete("evict")
         keep = min(keep, self.host.cols * self.host.page_rows)
         recent = min(recent, keep)
         kept = torch.empty(n, self.layers, self.ctx.hkv, keep, dtype=torch.int32, device=self.table.device)
