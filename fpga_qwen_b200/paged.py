@@ -133,7 +133,8 @@ class PagedSequences:
     A step's rows count from ``begin_step`` on, so until ``append`` has written them in every layer ``evict``, another
     ``begin_step`` and ``attend`` of a layer without them are refused (``QA_ERR_STATE``; closing the step's
     sequences ends it). Once an ``append`` has been captured into a graph the replays, which nothing here sees,
-    are taken to follow their ``begin_step`` at once: that order is then the caller's to keep.
+    are taken to follow their ``begin_step`` at once: that order is then the caller's to keep. Only ``append``
+    and ``attend`` can be captured; the calls that also keep the host's books are refused under capture.
     """
 
     def __init__(self, ctx: Context, n_pages: int, page_rows: int = 16, max_seqs: int = 1, max_rows: int = 4096,
@@ -161,6 +162,7 @@ class PagedSequences:
         return self.host.open()
 
     def close(self, seq: int):
+        self._check_uncaptured("close")
         self.host.close(seq)
         self.step.close(seq)
         self.lengths[seq] = 0
@@ -186,6 +188,15 @@ class PagedSequences:
     def _stream(self):
         self.ctx.set_stream(torch.cuda.current_stream(self.table.device).cuda_stream)
 
+    def _capturing(self) -> bool:
+        with torch.cuda.device(self.table.device):
+            return torch.cuda.is_current_stream_capturing()
+
+    def _check_uncaptured(self, what: str):
+        """A replay would repeat the device's part of these calls and not the host's books."""
+        if self._capturing():
+            raise QAttnError(QA_ERR_STATE, f"{what} while the stream is capturing")
+
     def _check_inputs(self, n, layers, **tensors):
         heads = {"q": self.ctx.hq, "k": self.ctx.hkv, "v": self.ctx.hkv}
         for name, t in tensors.items():
@@ -207,6 +218,7 @@ class PagedSequences:
         if n > self.ctx.config.context:
             raise QAttnError(QA_ERR_CAPACITY, "Context capacity exceeded")
         self._check_inputs(n, self.layers, q=q, k=k, v=v)
+        self._check_uncaptured("prefill")
         self._grow({seq: n})
         try:
             self._stream()
@@ -241,6 +253,7 @@ class PagedSequences:
         if not live:
             raise QAttnError(QA_ERR_STATE, "no open sequence")
         self.step.check_complete("begin_step")
+        self._check_uncaptured("begin_step")
         self._grow({seq: 1 for seq in live})
         self.step.begin(live)
         held = [self.host.rows[seq] for seq in range(len(self.host.pages))]
@@ -257,10 +270,8 @@ class PagedSequences:
         self.ctx.paged_append(self.pages, self.table.data_ptr(), n, self.host.cols, 0, self.lengths.data_ptr(),
                               self.positions.data_ptr(), n, layer, layers, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                               qn.data_ptr())
-        if not self.step.replays:
-            with torch.cuda.device(self.table.device):
-                if torch.cuda.is_current_stream_capturing():
-                    self.step.captured()
+        if not self.step.replays and self._capturing():
+            self.step.captured()
         self.step.wrote(layer, layers)
         return qn
 
@@ -284,6 +295,7 @@ class PagedSequences:
         if keep < 1 or not 0 <= recent <= keep:
             raise QAttnError(QA_ERR_INVALID, f"keep {keep}, recent {recent}")
         self.step.check_complete("evict")
+        self._check_uncaptured("evict")
         keep = min(keep, self.host.cols * self.host.page_rows)
         recent = min(recent, keep)
         kept = torch.empty(n, self.layers, self.ctx.hkv, keep, dtype=torch.int32, device=self.table.device)

@@ -122,3 +122,35 @@ def test_replayed_steps_are_the_callers_to_order():
         stream.synchronize()
         assert s.lengths.tolist() == [17, 17, 0] and s.positions.tolist() == [22, 35, 0] and out[:, :2].all()
         ctx.sync()
+
+
+def test_host_bookkeeping_is_refused_under_capture():
+    """A replay repeats the device's part alone: calls that also keep the host's books run outside a graph, and one made
+    inside changes neither side and leaves the capture valid."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ctx, s, draw = build((32, 33))
+        s.begin_step()
+        s.append(*draw(3))
+        q, k, v = draw(3)
+        qn, out = torch.empty_like(q), torch.zeros_like(q)
+        late, prompt = s.open(), draw(5)
+        before = state(s)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            refused(s.begin_step)
+            refused(lambda: s.evict(16))
+            refused(lambda: s.close(0))
+            refused(lambda: s.prefill(late, *prompt))
+            s.append(q, k, v, q_out=qn)
+            s.attend(qn, out=out)
+        assert same(before, state(s))
+        s.begin_step()
+        graph.replay()
+        stream.synchronize()
+        assert s.lengths.tolist() == [34, 35, 1] and out.all()
+        s.close(0)
+        s.evict(16)
+        assert [s.rows(b) for b in (1, late)] == [16, 1]
+        ctx.sync()
