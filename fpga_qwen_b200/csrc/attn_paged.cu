@@ -54,8 +54,12 @@
 // rows 8.6 -> 5.9 us, of 1024 rows 9.0 -> 8.0 us, 32 units of 2048 rows 13.7 -> 10.6 us, 144 units
 // of 512 rows 13.7 -> 8.4 us). Neither do calls of one sequence, long or not, whose units are equally
 // long: up to 148 of them have CTAs of their own, up to 296 half-size CTAs, two per SM
-// (paged_alone_equal: 224 units of 3970 rows 75.1 -> 68.5 us, 6.6 TB/s; with weights, of 2049 rows
-// 50.3 -> 42.0 us; 112 units of 8192 rows 78.1 -> 71.7 us).
+// (paged_alone_equal: 224 units of 3970 rows 75.1 -> 68.5 us; with weights, of 2049 rows 50.3 -> 42.0 us;
+// 112 units of 8192 rows 78.1 -> 71.7 us, all on the same inputs call after call. On inputs that change with every
+// call the first is 73 to 74 us, 6.2 TB/s, and the second 47.4 us with the reset of the weights, some 3 us).
+// Both rules go by the rows that the table can hold, since lengths are not known on the host; the figures are of
+// tables as narrow as the rows. 8 units of 452 rows take 7.3 us with a table of up to 1024 rows and 8.9 us, the
+// even split, with a wider one; 64 units of 256 rows 6.5 and 9.3 us.
 //
 // Every wait is bounded: on expiry the CTA records an error code, consumes no further block, and
 // drains its copies before it exits.

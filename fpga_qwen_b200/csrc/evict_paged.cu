@@ -328,7 +328,8 @@ cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t s) {
     const int per = (max_rows + ranks - 1) / ranks;
     if (per > MAX_SLICE) return cudaErrorInvalidValue;       // (refused before)
     // short tables: small CTAs, more of them per SM (6,496 units of 65 rows, both
-    // launches: 123 -> 61 us)
+    // launches: 123 -> 61 us; kept 33 of 65: 80 us with a table of 80 rows, 134 us with one of 4096 and 225 us with
+    // one of 32768, whose CTAs take the shared memory of a full row: lengths are not known on the host)
     const bool small = per <= 1024 && ranks == 1;
     const cudaError_t e = launch(small ? evict_select_kernel<128> : evict_select_kernel<512>, dim3(units), small ? 128 : 512,
                                  (size_t)per * sizeof(float), ranks, a.overlap, a, s);

@@ -123,11 +123,14 @@ class PagedSequences:
     """Up to max_seqs sequences of a context over a pool of n_pages pages.
 
     ``prefill`` runs a prompt in sequence slot `slot` of the context (the prefill kernels read
-    contiguous rows) and leaves its rows in pages; ``begin_step``, then ``append`` and ``attend``
-    per layer (or for all layers), make one decode step of every open sequence; ``evict`` brings
-    them under a budget by accumulated attention weight. ``max_position`` bounds RoPE positions,
-    which go on past the cached rows once rows are evicted; ``step_layers`` is the most layers of one
-    ``attend`` call (it sizes the workspace, which is made once, so that captured steps stay valid).
+    contiguous rows; what the slot held before is gone) and leaves its rows in pages; ``begin_step``,
+    then ``append`` and ``attend`` per layer (or for all layers), make one decode step of every open
+    sequence; ``evict`` brings them under a budget by accumulated attention weight. ``max_position``
+    bounds RoPE positions, which go on past the cached rows once rows are evicted; ``step_layers`` is the
+    most layers of one ``attend`` call (it sizes the workspace, which is made once, so that captured steps
+    stay valid: 8 bytes for every sequence, layer, KV head and row; 1 is enough for a loop over layers).
+    The constructor extends the context's RoPE tables where ``max_position`` is past them, after which
+    graphs captured on the context before have to be captured again (``qa_rope_positions``).
     One caller, and one stream, at a time, as for the context.
 
     A step's rows count from ``begin_step`` on, so until ``append`` has written them in every layer ``evict``, another
@@ -289,8 +292,10 @@ class PagedSequences:
 
     def evict(self, keep: int, recent: int = 0):
         """Every sequence of more than `keep` cached rows keeps its last `recent` rows and the heaviest
-        others, in each layer and head; their pages past that return to the pool. Returns the old
-        indices of the kept rows, [max_seqs][L][hkv][keep] (-1: none)."""
+        others, in each layer and head; their pages past that return to the pool. A row's weight is what
+        ``attend`` calls since its append gave it: rows of a prompt weigh nothing until then, and of rows that
+        weigh the same the older stay. Returns the old indices of the kept rows,
+        [max_seqs][L][hkv][keep] (-1: none)."""
         n = self.table.shape[0]
         if keep < 1 or not 0 <= recent <= keep:
             raise QAttnError(QA_ERR_INVALID, f"keep {keep}, recent {recent}")

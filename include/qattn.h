@@ -319,8 +319,8 @@ int qa_paged_attn(qa_ctx* ctx, const qa_pages* pages, const int* table, int tabl
  * The kept rows move, in their order, with their weights, to rows [0, keep) of dst_table's row b.
  * Sequences of at most `keep` rows keep all of them. All layers of the context.
  *   src_table [n][src_cols], dst_table [n][dst_cols], lengths [n], new_lengths [n]: device ints.
- * In place: dst_table names the same pages (it may be src_table itself, and new_lengths may be
- * lengths); otherwise a sequence's dst pages are disjoint from every src page of the call. No two
+ * In place: dst_table names the same pages in the same columns (it may be src_table itself, and
+ * new_lengths may be lengths); otherwise a sequence's dst pages are disjoint from every src page of the call. No two
  * sequences share a dst page; in place, src pages are not shared either. new_lengths[b] =
  * min(lengths[b], keep). kept: device, [n][n_layers][hkv_local][keep] ints, receives each kept
  * row's old index (ascending; -1 past new_lengths[b]). Rows of dst pages past new_lengths[b] are
